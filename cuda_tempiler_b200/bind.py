@@ -113,22 +113,63 @@ def covered_w8a16(x2, W, scale, zero, group_size) -> bool:
 
 
 # ------------------------------------------------------------------------------ linear layers
-def linear_fp16(x: torch.Tensor, weight: torch.Tensor,
-                bias: torch.Tensor | None = None) -> torch.Tensor:
-    """y = x @ weight^T (+ bias) for x [..., K], weight [N, K]."""
+def _stock_epilogue(y, activation, residual):
+    """The epilogue of the stock path, on the layer's fp16 output."""
+    if activation not in ops.ACTIVATIONS:
+        raise ValueError(f"activation {activation!r}")
+    if activation == "relu":
+        y = F.relu(y)
+    elif activation == "silu":
+        y = F.silu(y)
+    elif activation in ("gelu", "gelu_tanh"):
+        y = F.gelu(y, approximate="tanh" if activation == "gelu_tanh" else "none")
+    return y if residual is None else y + residual
+
+
+def _fused(x2, N, bias, activation, residual, run):
+    """run(residual rows) where the epilogue kernels cover the extra operands, else None."""
+    res = None if residual is None else residual.reshape(-1, N)
+    if res is not None and (res.dtype != torch.float16 or res.device != x2.device
+                            or res.shape[0] != x2.shape[0] or res.stride(1) != 1
+                            or res.stride(0) % 8 or not _aligned(res)):
+        return None
+    if bias is not None and (bias.dtype != torch.float16 or bias.device != x2.device
+                             or not bias.is_contiguous() or not _aligned(bias)):
+        return None
+    try:
+        return run(res)
+    except NotCovered:
+        return None
+
+
+def linear_fp16(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                activation: str | None = None,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
+    """y = act(x @ weight^T (+ bias)) (+ residual) for x [..., K], weight [N, K], residual
+    [..., N].  With an activation or a residual the kernels fuse the whole epilogue
+    (``ops.gemm_fp16_epilogue``); a bias alone is added to the rounded product."""
+    fuse = activation not in (None, "none") or residual is not None
     if enabled():
         x2 = x.reshape(-1, x.shape[-1])
         if covered_fp16(x2, weight):
-            try:
-                y = torch.ops.tempo.gemm_fp16(x2, weight)
-            except NotCovered:
-                y = None
-            if y is not None:
-                _count("tempo")
-                y = y.reshape(*x.shape[:-1], weight.shape[0])
-                return y + bias if bias is not None else y
+            N = weight.shape[0]
+            if fuse:
+                y = _fused(x2, N, bias, activation, residual, lambda res: ops.gemm_fp16_epilogue(
+                    x2, weight, bias, activation, res))
+                if y is not None:
+                    _count("tempo")
+                    return y.reshape(*x.shape[:-1], N)
+            else:
+                try:
+                    y = torch.ops.tempo.gemm_fp16(x2, weight)
+                except NotCovered:
+                    y = None
+                if y is not None:
+                    _count("tempo")
+                    y = y.reshape(*x.shape[:-1], N)
+                    return y + bias if bias is not None else y
     _count("fallback")
-    return F.linear(x, weight, bias)
+    return _stock_epilogue(F.linear(x, weight, bias), activation, residual)
 
 
 def dequantize(W, scale, zero=None, group_size: int = 0) -> torch.Tensor:
@@ -143,17 +184,29 @@ def dequantize(W, scale, zero=None, group_size: int = 0) -> torch.Tensor:
 
 def linear_w8a16(x: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
                  zero: torch.Tensor | None = None, group_size: int = 0,
-                 bias: torch.Tensor | None = None) -> torch.Tensor:
+                 bias: torch.Tensor | None = None, activation: str | None = None,
+                 residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``linear_fp16`` with an 8-bit weight."""
+    fuse = activation not in (None, "none") or residual is not None
     if enabled():
         x2 = x.reshape(-1, x.shape[-1])
         if covered_w8a16(x2, W, scale, zero, group_size):
-            try:
-                y = torch.ops.tempo.gemm_w8a16(x2, W, scale, zero, group_size)
-            except NotCovered:
-                y = None
-            if y is not None:
-                _count("tempo")
-                y = y.reshape(*x.shape[:-1], W.shape[0])
-                return y + bias if bias is not None else y
+            N = W.shape[0]
+            if fuse:
+                y = _fused(x2, N, bias, activation, residual, lambda res: ops.gemm_w8a16_epilogue(
+                    x2, W, scale, zero, group_size, bias, activation, res))
+                if y is not None:
+                    _count("tempo")
+                    return y.reshape(*x.shape[:-1], N)
+            else:
+                try:
+                    y = torch.ops.tempo.gemm_w8a16(x2, W, scale, zero, group_size)
+                except NotCovered:
+                    y = None
+                if y is not None:
+                    _count("tempo")
+                    y = y.reshape(*x.shape[:-1], N)
+                    return y + bias if bias is not None else y
     _count("fallback")
-    return F.linear(x, dequantize(W, scale, zero, group_size), bias)
+    return _stock_epilogue(F.linear(x, dequantize(W, scale, zero, group_size), bias), activation,
+                           residual)

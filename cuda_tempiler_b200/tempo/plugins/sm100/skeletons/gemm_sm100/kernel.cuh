@@ -30,6 +30,20 @@ namespace tempo_sm100 {
 
 enum WeightQuant : int { kWFp16 = 0, kWInt8PerChannel = 1, kWUint8Group = 2 };
 
+// Epilogue of the EPI instantiations: y = act(acc * scale[n] + bias[n]) + res[m][n], in fp32 on
+// the accumulator, rounded once to fp16.  Null pointers leave their term out.  Every load is 16
+// bytes of 8 columns (N % 8 == 0, 16-byte aligned), made where the accumulator already is: the
+// separate pass it replaces reads and writes C once more (4 M N bytes).
+enum EpiAct : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
+
+struct EpiArgs {
+  const __half* scale = nullptr;  // per output channel (weights expanded without their scale)
+  const __half* bias = nullptr;   // [N]
+  const __half* res = nullptr;    // [M][N], may be C itself
+  long long ldr = 0;              // row stride of res in elements
+  int act = kActNone;
+};
+
 struct GemmArgs {
   int rows_p, rows_q, K;
   int tiles_p, tiles_q, num_kb, splits, num_units;
@@ -52,6 +66,7 @@ struct GemmArgs {
   int sk_tile0;         // first tail tile
   int sk_tiles;         // tail tiles
   int sk_splits;        // k-slices per tail tile
+  EpiArgs epi;          // EPI instantiations only
 };
 
 __host__ __device__ constexpr int round_up(int x, int a) { return (x + a - 1) / a * a; }
@@ -190,7 +205,67 @@ __device__ __forceinline__ void acc_chunk(uint32_t t_acc, int c, float (&f)[32])
   }
 }
 
-template <int BN, int WQ, bool SWAP, bool SMEMDQ = false>
+__device__ __forceinline__ float epi_act(float x, int act) {
+  switch (act) {
+    case kActRelu: return x > 0.f || x != x ? x : 0.f;  // NaN passes through
+    case kActSilu: return x / (1.f + expf(-x));
+    case kActGelu: return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+    case kActGeluTanh:
+      return 0.5f * x * (1.f + tanhf(0.79788456080286536f * (x + 0.044715f * x * x * x)));
+    default: return x;
+  }
+}
+
+__device__ __forceinline__ void unpack_half8(uint4 v, float (&f)[8]) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = __half22float2(h[i]);
+    f[2 * i] = x.x;
+    f[2 * i + 1] = x.y;
+  }
+}
+
+// The epilogue of columns [n0, n0 + 32) of row m held by one thread.  The residual is read with
+// plain loads: C may be the same memory, and this thread reads an element before anyone writes it.
+__device__ __forceinline__ void epi_row32(const EpiArgs& e, float (&f)[32], int m, int m_rows,
+                                          int n0, int n_cols) {
+  if (m >= m_rows) return;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int n = n0 + 8 * g;
+    if (n >= n_cols) break;
+    float v[8];
+    if (e.scale) {
+      unpack_half8(__ldg(reinterpret_cast<const uint4*>(e.scale + n)), v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[8 * g + i] *= v[i];
+    }
+    if (e.bias) {
+      unpack_half8(__ldg(reinterpret_cast<const uint4*>(e.bias + n)), v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[8 * g + i] += v[i];
+    }
+    if (e.act != kActNone) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[8 * g + i] = epi_act(f[8 * g + i], e.act);
+    }
+    if (e.res) {
+      unpack_half8(*reinterpret_cast<const uint4*>(e.res + (long long)m * e.ldr + n), v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[8 * g + i] += v[i];
+    }
+  }
+}
+
+// One element (row m, column n) of the epilogue; b is bias[n] as a float (0 without a bias).
+__device__ __forceinline__ float epi_one(const EpiArgs& e, float v, float b, int m, int n) {
+  v = epi_act(v + b, e.act);
+  if (e.res) v += __half2float(e.res[(long long)m * e.ldr + n]);
+  return v;
+}
+
+template <int BN, int WQ, bool SWAP, bool SMEMDQ = false, bool EPI = false>
 __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
     k_gemm_sm100(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                  const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapC,
@@ -557,6 +632,17 @@ __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
               acc.z *= __half2float(__ldg(args.scale + n + 2));
               acc.w *= __half2float(__ldg(args.scale + n + 3));
             }
+            if (EPI) {
+              float b[4] = {0.f, 0.f, 0.f, 0.f};
+              if (args.epi.bias) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] = __half2float(__ldg(args.epi.bias + n + i));
+              }
+              acc.x = epi_one(args.epi, acc.x, b[0], m, n);
+              acc.y = epi_one(args.epi, acc.y, b[1], m, n + 1);
+              acc.z = epi_one(args.epi, acc.z, b[2], m, n + 2);
+              acc.w = epi_one(args.epi, acc.w, b[3], m, n + 3);
+            }
             uint2 w;
             w.x = pack_half2(acc.x, acc.y);
             w.y = pack_half2(acc.z, acc.w);
@@ -596,6 +682,7 @@ __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
               f[j] *= __half2float(q < args.weight_rows ? __ldg(args.scale + q) : __half(0.f));
             }
           }
+          if (EPI) epi_row32(args.epi, f, p, args.rows_p, q0 + c * 32, args.rows_q);
           if (lane == 0) bulk_wait_group_read<1>();
           __syncwarp();
           uint8_t* sbuf = stage_buf + sb * 2048;
@@ -621,6 +708,8 @@ __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
         // swapped: C[q][p]; lanes run along p (= n), so each column store is coalesced.
         const float sc =
             (WQ == kWInt8PerChannel && p < args.rows_p) ? __half2float(__ldg(args.scale + p)) : 1.f;
+        const float bias = (EPI && args.epi.bias && p < args.rows_p)
+                               ? __half2float(__ldg(args.epi.bias + p)) : 0.f;
 #pragma unroll 1
         for (int c = 0; c < BN / Cfg::CW; ++c) {
           float f[32];
@@ -634,8 +723,11 @@ __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
 #pragma unroll
             for (int j = 0; j < Cfg::CW; ++j) {
               const int q = q0 + c * Cfg::CW + j;
-              if (q < args.rows_q)
-                args.C[(long long)q * args.ldc + p] = __float2half_rn(f[j] * sc);
+              if (q < args.rows_q) {
+                float v = f[j] * sc;
+                if (EPI) v = epi_one(args.epi, v, bias, q, p);
+                args.C[(long long)q * args.ldc + p] = __float2half_rn(v);
+              }
             }
           }
         }
@@ -1395,7 +1487,7 @@ struct PairCfg {
   static_assert(2 * STAGES + 5 <= BAR_BYTES / 8 - 2, "barrier area too small");
 };
 
-template <int BN, bool SWIGLU>
+template <int BN, bool SWIGLU, bool EPI = false>
 __global__ void __launch_bounds__(PairCfg<BN>::THREADS, 1)
     k_gemm_sm100_pair(const __grid_constant__ CUtensorMap mapA,
                       const __grid_constant__ CUtensorMap mapB,
@@ -1652,6 +1744,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::THREADS, 1)
             if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(buf), 0));
           }
           if (p >= args.rows_p) continue;
+          if (EPI) epi_row32(args.epi, acc, p, args.rows_p, q0 + c * 32, args.rows_q);
 #pragma unroll
           for (int i0 = 0; i0 < 32; i0 += 8) {
             const int q = q0 + c * 32 + i0;
@@ -1724,6 +1817,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::THREADS, 1)
           if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(buf), 0));
         }
         if (!rows_live) continue;
+        if (EPI) epi_row32(args.epi, f, row0 + lane, args.rows_p, q0 + c * 32, args.rows_q);
         if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
         uint8_t* sbuf = stage_buf + sb * 2048;
@@ -1814,7 +1908,7 @@ struct PairW8Cfg {
   static_assert(SMEM <= kMaxDynSmem, "shared memory");
 };
 
-template <int BN, int WQ>
+template <int BN, int WQ, bool EPI = false>
 __global__ void __launch_bounds__(PairW8Cfg<BN>::THREADS, 1)
     k_gemm_sm100_pair_w8(const __grid_constant__ CUtensorMap mapA,
                          const __grid_constant__ CUtensorMap mapW,
@@ -2164,11 +2258,13 @@ __global__ void __launch_bounds__(PairW8Cfg<BN>::THREADS, 1)
             if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(buf), 0));
           }
           if (p >= args.rows_p) continue;
+          // EPI instantiations take the per-channel scale as epi.scale
+          if (EPI) epi_row32(args.epi, acc, p, args.rows_p, q0 + c * 32, args.rows_q);
 #pragma unroll
           for (int i0 = 0; i0 < 32; i0 += 8) {
             const int q = q0 + c * 32 + i0;
             if (q >= args.rows_q) break;
-            if (WQ == kWInt8PerChannel) {
+            if (WQ == kWInt8PerChannel && !EPI) {
 #pragma unroll
               for (int j = 0; j < 8; ++j)
                 acc[i0 + j] *= q + j < args.rows_q ? __half2float(__ldg(args.scale + q + j)) : 0.f;
@@ -2190,7 +2286,7 @@ __global__ void __launch_bounds__(PairW8Cfg<BN>::THREADS, 1)
       for (int c = 0; c < nchunk; ++c) {
         float f[32];
         acc_chunk<32, 1, BN>(t_acc, c, f);
-        if (WQ == kWInt8PerChannel) {
+        if (WQ == kWInt8PerChannel && !EPI) {
           // per-output-channel scale of columns q0 + 32 c + j: lane j loads one, all share it
           const int n = q0 + c * 32 + lane;
           const float sv = n < args.rows_q ? __half2float(__ldg(args.scale + n)) : 0.f;
@@ -2203,6 +2299,7 @@ __global__ void __launch_bounds__(PairW8Cfg<BN>::THREADS, 1)
           if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(buf), 0));
         }
         if (!rows_live) continue;
+        if (EPI) epi_row32(args.epi, f, row0 + lane, args.rows_p, q0 + c * 32, args.rows_q);
         if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
         uint8_t* sbuf = stage_buf + sb * 2048;

@@ -180,6 +180,7 @@ struct Problem {
   // prefill puts its expanded weights between the two, so that nothing but counters ever
   // occupies the prefix of a workspace a caller reuses across problems.
   void* ws_parts = nullptr;
+  EpiArgs epi = EpiArgs{};  // read by the EPI instantiations only
 };
 
 struct Hyper {
@@ -212,10 +213,12 @@ size_t ws_needed(int tiles, int splits, int bn) {
 // ------------------------------------------------------------------------------------------
 // Instantiation table.
 // ------------------------------------------------------------------------------------------
-template <int BN, int WQ, bool SWAP, bool SMEMDQ = false>
+// EPI: the instantiation with the fused epilogue (k-splits through the global workspace have none).
+template <int BN, int WQ, bool SWAP, bool SMEMDQ = false, bool EPI = false>
 cudaError_t launch_inst(const Problem& pr, const Hyper& h, cudaStream_t st) {
   using Cfg = SkelCfg<BN, WQ, SWAP, SMEMDQ>;
-  auto kern = k_gemm_sm100<BN, WQ, SWAP, SMEMDQ>;
+  auto kern = k_gemm_sm100<BN, WQ, SWAP, SMEMDQ, EPI>;
+  if (EPI && h.splits > kMaxClusterSplit) return cudaErrorInvalidConfiguration;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -258,6 +261,7 @@ cudaError_t launch_inst(const Problem& pr, const Hyper& h, cudaStream_t st) {
   a.group_size = pr.group > 0 ? pr.group : 1;
   a.groups_per_row = pr.group > 0 ? pr.K / pr.group : 1;
   a.weight_rows = pr.N;
+  if (EPI) a.epi = pr.epi;
 
   CUtensorMap mP, mQ, mW, mC, mS, mZ;
   std::memset(&mS, 0, sizeof(mS));
@@ -536,10 +540,11 @@ PairPlan pair_plan(int M, int N, int K, int bn, int sms, int max_ctas, bool spli
 
 // 2-CTA (cta_group::2) fp16 prefill launch: persistent clusters of two CTAs; h.splits > 1
 // allows the split tail of pair_plan.
-template <int BN, bool SWIGLU = false>
+template <int BN, bool SWIGLU = false, bool EPI = false>
 cudaError_t launch_pair(const Problem& pr, const Hyper& h, cudaStream_t st) {
   using Cfg = PairCfg<BN>;
-  auto kern = k_gemm_sm100_pair<BN, SWIGLU>;
+  static_assert(!(SWIGLU && EPI), "one epilogue");
+  auto kern = k_gemm_sm100_pair<BN, SWIGLU, EPI>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -572,6 +577,7 @@ cudaError_t launch_pair(const Problem& pr, const Hyper& h, cudaStream_t st) {
   a.C = static_cast<__half*>(pr.C);
   a.ldc = pr.ldc;
   a.weight_rows = pr.N;
+  if (EPI) a.epi = pr.epi;
   a.sk_tile0 = pl.sk_tile0;
   a.sk_tiles = pl.sk_tiles;
   a.sk_splits = pl.sk_splits;
@@ -597,10 +603,10 @@ cudaError_t launch_pair(const Problem& pr, const Hyper& h, cudaStream_t st) {
 
 // W8A16 2-CTA launch (k_gemm_sm100_pair_w8): persistent clusters; h.splits > 1 allows the
 // split tail of pair_plan (given the workspace it needs).
-template <int BN, int WQ>
+template <int BN, int WQ, bool EPI = false>
 cudaError_t launch_pair_w8(const Problem& pr, const Hyper& h, cudaStream_t st) {
   using Cfg = PairW8Cfg<BN>;
-  auto kern = k_gemm_sm100_pair_w8<BN, WQ>;
+  auto kern = k_gemm_sm100_pair_w8<BN, WQ, EPI>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -636,6 +642,10 @@ cudaError_t launch_pair_w8(const Problem& pr, const Hyper& h, cudaStream_t st) {
   a.zero = static_cast<const uint8_t*>(pr.zero);
   a.group_size = pr.group > 0 ? pr.group : 1;
   a.groups_per_row = pr.group > 0 ? pr.K / pr.group : 1;
+  if (EPI) {
+    a.epi = pr.epi;
+    if (WQ == kWInt8PerChannel) a.epi.scale = static_cast<const __half*>(pr.scale);
+  }
   a.sk_tile0 = pl.sk_tile0;
   a.sk_tiles = pl.sk_tiles;
   a.sk_splits = pl.sk_splits;

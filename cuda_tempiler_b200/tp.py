@@ -201,11 +201,36 @@ class PeerAllReduce:
         self._own = []
 
 
+def _rank(group) -> int:
+    import torch.distributed as dist
+    return dist.get_rank(group) if dist.is_available() and dist.is_initialized() else 0
+
+
+def _down_residual(h, w, s, residual):
+    """The down GEMM with the residual in its epilogue."""
+    from . import ops
+    if w.dtype == torch.float16:
+        return ops.gemm_fp16_epilogue(h, w, residual=residual)
+    return ops.gemm_w8a16_epilogue(h, w, s, residual=residual)
+
+
+def _sum_partial(y, group, all_reduce):
+    if callable(all_reduce):                              # e.g. a PeerAllReduce
+        return all_reduce(y)
+    if all_reduce:
+        import torch.distributed as dist
+        if dist.is_available() and dist.is_initialized() and dist.get_world_size(group) > 1:
+            dist.all_reduce(y, op=dist.ReduceOp.SUM, group=group)
+    return y
+
+
 def mlp_forward(x: torch.Tensor, shard: MLPShard, group=None, gemm=None, swiglu=None,
-                all_reduce=True, fused=None) -> torch.Tensor:
+                all_reduce=True, fused=None, residual: torch.Tensor | None = None) -> torch.Tensor:
     """y = down(silu(gate(x)) * up(x)) for this rank's shard, summed over the group.  With the
     library's own GEMM (gemm None) and an interleaved shard the fused gate_up + SwiGLU kernel
-    runs where it covers M; ``fused=False`` keeps the two-kernel path."""
+    runs where it covers M; ``fused=False`` keeps the two-kernel path.  ``residual`` [M, H] is added
+    once: by rank 0 to its partial, in the down GEMM's epilogue."""
+    own_gemm = gemm is None
     if fused is None:
         fused = _default_fused if gemm is None else False
     gemm = gemm or _default_gemm
@@ -214,14 +239,52 @@ def mlp_forward(x: torch.Tensor, shard: MLPShard, group=None, gemm=None, swiglu=
     if h is None:
         gu = gemm(x, shard.w_gate_up, shard.s_gate_up)   # [M, 2 I/tp]
         h = swiglu(gu, shard.gu_block)                    # [M, I/tp]
-    y = gemm(h, shard.w_down, shard.s_down)               # [M, H] partial
-    if callable(all_reduce):                              # e.g. a PeerAllReduce
-        return all_reduce(y)
-    if all_reduce:
-        import torch.distributed as dist
-        if dist.is_available() and dist.is_initialized() and dist.get_world_size(group) > 1:
-            dist.all_reduce(y, op=dist.ReduceOp.SUM, group=group)
-    return y
+    if residual is not None and _rank(group) == 0:
+        if own_gemm:
+            y = _down_residual(h, shard.w_down, shard.s_down, residual)
+        else:
+            y = gemm(h, shard.w_down, shard.s_down) + residual
+    else:
+        y = gemm(h, shard.w_down, shard.s_down)           # [M, H] partial
+    return _sum_partial(y, group, all_reduce)
+
+
+@dataclass
+class MoEShard:
+    """One rank's slice of every expert: gate and up rows [r I/tp, (r+1) I/tp) stacked as
+    [E, 2 I/tp, H], the matching columns of the down weights [E, H, I/tp]; scales per output row
+    (int8) or None (fp16)."""
+    w_gate_up: torch.Tensor
+    s_gate_up: torch.Tensor | None
+    w_down: torch.Tensor
+    s_down: torch.Tensor | None
+
+
+def shard_moe(w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, world: int,
+              rank: int, s_gate=None, s_up=None, s_down=None) -> MoEShard:
+    """Cut full expert weights (gate / up [E, I, H], down [E, H, I]) into rank `rank`'s slices: for
+    a few tokens every rank reads 1 / tp of each expert that is reached, whichever they are."""
+    sl = shard_rows(w_gate.shape[1], world, rank)
+    sgu = None if s_gate is None else torch.cat([s_gate[:, sl], s_up[:, sl]], 1).contiguous()
+    return MoEShard(torch.cat([w_gate[:, sl], w_up[:, sl]], 1).contiguous(), sgu,
+                    w_down[:, :, sl].contiguous(), s_down)
+
+
+def _default_layer(x, w_router, shard, top_k, normalize, residual):
+    from . import ops
+    return ops.moe_layer(x, w_router, shard.w_gate_up, shard.w_down, top_k, normalize,
+                         s_gate_up=shard.s_gate_up, s_down=shard.s_down, residual=residual)
+
+
+def moe_forward(x: torch.Tensor, w_router: torch.Tensor, shard: MoEShard, top_k: int,
+                normalize: bool = True, group=None, layer=None, all_reduce=True,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
+    """The mixture-of-experts layer of ``ops.moe_layer`` over the ranks of the group: every rank
+    routes (the router is not sharded), runs its slice of the chosen experts, and the fp16 partials
+    are summed; ``residual`` is added by rank 0."""
+    layer = layer or _default_layer
+    y = layer(x, w_router, shard, top_k, normalize, residual if _rank(group) == 0 else None)
+    return _sum_partial(y, group, all_reduce)
 
 
 class MLPGraph:

@@ -142,6 +142,67 @@ int tempo_sm100_gemm_w8a16_swiglu(const void* A, const void* W, const void* scal
                                   int ldc, int quant_kind, int group_size, void* ws,
                                   size_t ws_bytes, void* stream);
 
+/* GEMM with a fused epilogue: C = act(A W^T + bias) + residual, the epilogue in fp32 on the
+ * accumulator and one rounding to fp16.  Layouts, strides, coverage and return codes of
+ * tempo_sm100_gemm_fp16 / tempo_sm100_gemm_w8a16; workspace as tempo_sm100_workspace_bytes says.
+ * bias: fp16 [N] or NULL.  residual: fp16 [M][N], row stride ldr elements, or NULL; it may be C
+ * itself (same pointer and stride), no other overlap.  bias, residual and (W8A16) scale 16-byte
+ * aligned, ldr a multiple of 8 (else 9).  activation: a TEMPO_ACT_* value (else 1). */
+#define TEMPO_ACT_NONE 0
+#define TEMPO_ACT_RELU 1
+#define TEMPO_ACT_SILU 2
+#define TEMPO_ACT_GELU 3       /* x Phi(x) */
+#define TEMPO_ACT_GELU_TANH 4  /* its tanh approximation */
+int tempo_sm100_gemm_fp16_epilogue(const void* A, const void* B, void* C, const void* bias,
+                                   const void* residual, int M, int N, int K, int lda, int ldb,
+                                   int ldc, int ldr, int activation, void* ws, size_t ws_bytes,
+                                   void* stream);
+int tempo_sm100_gemm_w8a16_epilogue(const void* A, const void* W, const void* scale,
+                                    const void* zero, void* C, const void* bias,
+                                    const void* residual, int M, int N, int K, int lda, int ldw,
+                                    int ldc, int ldr, int quant_kind, int group_size,
+                                    int activation, void* ws, size_t ws_bytes, void* stream);
+
+/* Mixture-of-experts routing: logits = x w_router^T (+ bias), fp32; the top_k largest of each
+ * token in descending order (equal logits: the lower expert first) and their softmax weights,
+ * over the chosen experts (normalize != 0) or over all.  x [T][H] fp16 (row stride ldx),
+ * w_router [E][H] fp16 (ldw), bias fp16 [E] or NULL; ids [T][top_k], weights [T][top_k] dense.
+ * Any T; E <= 512, top_k <= min(16, E), H and strides multiples of 8, x and w_router 16-byte
+ * aligned (else 9).  A NaN logit ranks last and makes all weights of its token NaN. */
+int tempo_sm100_moe_route(const void* x, const void* w_router, const void* bias, int* ids,
+                          float* weights, int T, int E, int H, int top_k, int ldx, int ldw,
+                          int normalize, void* stream);
+
+/* A whole mixture-of-experts layer for up to 32 tokens:
+ *   y[t] = residual[t] + sum_j w[t][j] down_e(silu(gate_e(x_t)) * up_e(x_t)), e = ids[t][j]
+ * with ids and weights as tempo_sm100_moe_route computes them (and written out).  Each expert
+ * that a token chose is read once.  weight_kind 0: fp16; else a TEMPO_W8_* kind.
+ * w_gate_up [E][2I][H], w_down [E][H][I], dense.  gu_block 0: gate rows [0, I), up rows [I, 2I);
+ * b > 0: gate and up rows alternate in blocks of b (as tempo_sm100_silu_mul's columns).
+ * Scales: int8 s_gate_up [E][2I], s_down [E][H]; uint8 s / z_gate_up [E][H/group][2I],
+ * s / z_down [E][I/group][H].  H and I multiples of 16, group_size a multiple of 64 dividing
+ * both, gu_block a multiple of 8 dividing I, top_k <= 16, E <= 512 (else 9).  residual may be y
+ * itself, or NULL.  ws: tempo_sm100_moe_workspace_bytes, 16-byte aligned, any contents; calls
+ * that can run at the same time need one each. */
+size_t tempo_sm100_moe_workspace_bytes(int T, int top_k, int I);
+int tempo_sm100_moe_layer(const void* x, const void* w_router, const void* bias,
+                          const void* w_gate_up, const void* w_down, const void* s_gate_up,
+                          const void* z_gate_up, const void* s_down, const void* z_down,
+                          const void* residual, void* y, int* ids, float* weights, int T, int E,
+                          int H, int I, int top_k, int ldx, int ldw, int ldr, int ldy,
+                          int weight_kind, int group_size, int gu_block, int normalize, void* ws,
+                          size_t ws_bytes, void* stream);
+
+/* The same with the caller's routing: ids [T][top_k], weights [T][top_k] dense.  An id outside
+ * [0, E) names no expert (a token with none gets its residual, or zero); an expert named twice by
+ * a token counts with the sum of the two weights. */
+int tempo_sm100_moe_experts(const void* x, const int* ids, const float* weights,
+                            const void* w_gate_up, const void* w_down, const void* s_gate_up,
+                            const void* z_gate_up, const void* s_down, const void* z_down,
+                            const void* residual, void* y, int T, int E, int H, int I, int top_k,
+                            int ldx, int ldr, int ldy, int weight_kind, int group_size,
+                            int gu_block, void* ws, size_t ws_bytes, void* stream);
+
 /* Peer memory for the tensor-parallel exchange (one process per GPU of one node): a zeroed
  * device allocation of its own (an IPC handle maps a whole allocation, so the buffers must not
  * be sub-allocations of a caching allocator) and its release, the 64-byte CUDA IPC handle of

@@ -1,0 +1,257 @@
+"""GPU parity of the GEMM with a fused epilogue against its 64-bit restatement: every path (the
+weight stream, the 1-CTA tiles with and without a k-split, the 2-CTA tiles with and without a
+split tail, the expanded prefill), every activation, ragged sizes, strides, in-place residuals."""
+import itertools
+
+import pytest
+import torch
+
+from oracle import layer_oracle as L
+
+pytestmark = pytest.mark.gpu
+
+
+def weights(kind, N, K, group, seed=0):
+    g = torch.Generator("cuda").manual_seed(seed + 1000)
+    if kind == "fp16":
+        return (torch.randn(N, K, generator=g, device="cuda") * K ** -0.5).half(), None, None
+    if kind == "int8":
+        W = torch.randint(-128, 128, (N, K), generator=g, device="cuda", dtype=torch.int8)
+        return W, ((torch.rand(N, generator=g, device="cuda") + 0.5) * K ** -0.5 / 73).half(), None
+    W = torch.randint(0, 256, (N, K), generator=g, device="cuda", dtype=torch.uint8)
+    s = ((torch.rand(K // group, N, generator=g, device="cuda") + 0.5) * K ** -0.5 / 74).half()
+    z = torch.randint(0, 256, (K // group, N), generator=g, device="cuda", dtype=torch.uint8)
+    return W, s, z
+
+
+def rand(*shape, seed=0, scale=1.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).half()
+
+
+def call(A, w, group, **kw):
+    from cuda_tempiler_b200 import ops
+    W, s, z = w
+    if s is None:
+        return ops.gemm_fp16_epilogue(A, W, **kw)
+    return ops.gemm_w8a16_epilogue(A, W, s, z, group, **kw)
+
+
+def check(y, A, w, group, bias, act, res):
+    rounding = L.U16 if w[2] is not None and A.shape[0] > 16 else 0.0
+    ref, tol = L.epilogue(A, L.dequant(*w, group), bias, act, res, rounding)
+    bad = ((y.double() - ref).abs() > tol) | ~torch.isfinite(y)
+    assert not bad.any(), (int(bad.sum()), float(((y.double() - ref).abs() / tol).max()))
+
+
+def poison(M, N):
+    out = torch.empty(M, N, dtype=torch.float16, device="cuda")
+    out.view(torch.int16).fill_(0x7F7F)
+    return out
+
+
+KINDS = [("fp16", 0), ("int8", 0), ("uint8", 64), ("uint8", 128)]
+# rows of every band of the dispatch, with N and K ragged against every tile
+SHAPES = [(1, 8, 16), (1, 136, 272), (2, 1000, 528), (3, 2504, 1040), (8, 5008, 784),
+          (9, 264, 2064), (16, 9480, 400), (17, 272, 1040), (33, 1040, 2064), (64, 528, 4112),
+          (65, 784, 1040), (100, 2064, 528), (128, 1296, 784), (129, 1040, 2064), (200, 528, 4112),
+          (256, 4112, 272), (257, 784, 1040), (333, 2064, 2064), (600, 528, 4112),
+          (1025, 1040, 1296)]
+
+
+@pytest.mark.parametrize("kind,group", KINDS)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_shapes(dev, kind, group, M, N, K):
+    if group:
+        K = max(group, K // group * group)
+        N = -(-N // 16) * 16
+    A, w = rand(M, K, seed=M), weights(kind, N, K, group, seed=N)
+    bias, res = rand(N, seed=3), rand(M, N, seed=4)
+    out = poison(M, N)
+    y = call(A, w, group, bias=bias, activation="silu", residual=res, out=out)
+    assert y is out
+    check(y, A, w, group, bias, "silu", res)
+
+
+@pytest.mark.parametrize("kind,group", [("fp16", 0), ("int8", 0), ("uint8", 128)])
+@pytest.mark.parametrize("M", [1, 12, 40, 96, 160, 300])
+@pytest.mark.parametrize("act", L.ACT)
+def test_activations_and_terms(dev, kind, group, M, act):
+    N, K = 400, 512
+    A, w = rand(M, K, seed=M, scale=3.0), weights(kind, N, K, group)
+    for has_b, has_r in itertools.product((False, True), repeat=2):
+        bias = rand(N, seed=3) if has_b else None
+        res = rand(M, N, seed=4) if has_r else None
+        check(call(A, w, group, bias=bias, activation=act, residual=res), A, w, group, bias, act,
+              res)
+
+
+@pytest.mark.parametrize("kind,group", [("fp16", 0), ("int8", 0), ("uint8", 128)])
+@pytest.mark.parametrize("M", [5, 16, 50, 128, 256, 700, 1100])
+def test_strides_and_in_place(dev, kind, group, M):
+    """Row strides wider than the rows (what lies between stays as it was), the residual stream
+    updated in place."""
+    N, K = 656, 1152
+    A = rand(M, K + 24, seed=1)[:, :K]
+    w = list(weights(kind, N, K, group))
+    wide = torch.zeros(N, K + 32, dtype=w[0].dtype, device="cuda")
+    wide[:, :K] = w[0]
+    w[0] = wide[:, :K]
+    buf = rand(M + 2, N + 16, seed=2)
+    keep = buf.clone()
+    x = buf[1:M + 1, 8:N + 8]
+    call(A, w, group, residual=x, out=x)
+    check(x, A, (w[0].contiguous(), *w[1:]), group, None, "none", keep[1:M + 1, 8:N + 8])
+    keep[1:M + 1, 8:N + 8] = x
+    assert torch.equal(buf, keep)
+
+
+@pytest.mark.parametrize("M,N,K", [(300, 768, 8192), (512, 3840, 4096), (2048, 3840, 1024)])
+def test_split_tail(dev, M, N, K):
+    """Shapes whose last wave runs as k-slices: the epilogue applies once, to the whole sum."""
+    A, w = rand(M, K, seed=5), weights("fp16", N, K, 0)
+    bias, res = rand(N, seed=6), rand(M, N, seed=7)
+    for _ in range(2):
+        check(call(A, w, 0, bias=bias, activation="relu", residual=res), A, w, 0, bias, "relu", res)
+
+
+@pytest.mark.parametrize("kind,group", [("fp16", 0), ("int8", 0), ("uint8", 64)])
+@pytest.mark.parametrize("M", [1, 7, 16])
+def test_infinite_rows_stay_apart(dev, kind, group, M):
+    """An infinite or NaN activation reaches its own row only."""
+    N, K = 264 if kind != "uint8" else 272, 512
+    A, w = rand(M, K, seed=8), weights(kind, N, K, group)
+    clean = call(A, w, group)
+    A2 = A.clone()
+    A2[0, 3] = float("inf")
+    A2[M // 2, K - 1] = float("nan")
+    y = call(A2, w, group)
+    hit = {0, M // 2}
+    rest = [m for m in range(M) if m not in hit]
+    assert torch.equal(y[rest], clean[rest])
+    assert torch.isnan(y[M // 2]).all() and not torch.isfinite(y[0]).any()
+
+
+def test_extremes_of_the_activations(dev):
+    """relu keeps NaN, large arguments neither overflow nor lose their sign."""
+    from cuda_tempiler_b200 import ops
+    K, N = 16, 8
+    A = torch.zeros(6, K, dtype=torch.float16, device="cuda")
+    A[:, 0] = torch.tensor([60000.0, -60000.0, 30.0, -30.0, float("nan"), 0.0])
+    B = torch.zeros(N, K, dtype=torch.float16, device="cuda")
+    B[:, 0] = 1.0
+    for M, act in itertools.product((6, 48), L.ACT):
+        X = A.repeat(M // 6, 1)
+        y = ops.gemm_fp16_epilogue(X, B, activation=act)
+        ref = L.act(X[:, :1].double().expand(M, N), act)
+        assert torch.isnan(y[4::6]).all(), act
+        y, ref = y.double(), ref
+        keep = [i for i in range(M) if i % 6 != 4]
+        assert torch.allclose(y[keep], ref[keep], rtol=2.0 ** -10, atol=2.0 ** -23), act
+
+
+def test_results_do_not_change_between_runs(dev):
+    for kind, group, M in (("fp16", 0, 3), ("uint8", 128, 16), ("int8", 0, 90), ("fp16", 0, 512)):
+        A, w = rand(M, 2048, seed=9), weights(kind, 1040, 2048, group)
+        y = call(A, w, group, activation="gelu")
+        for _ in range(5):
+            assert torch.equal(y, call(A, w, group, activation="gelu"))
+
+
+@pytest.mark.parametrize("kind,group,M", [("fp16", 0, 4), ("fp16", 0, 300), ("int8", 0, 1100),
+                                          ("uint8", 128, 200)])
+def test_graph_capture(dev, kind, group, M):
+    """Two graphs captured on one stream replay with their own workspaces, on other streams."""
+    N, K = 3840, 2048
+    A, w = rand(M, K, seed=10), weights(kind, N, K, group)
+    res = [rand(M, N, seed=11 + i) for i in range(2)]
+    want = [call(A, w, group, residual=r) for r in res]
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        call(A, w, group, residual=res[0])
+    side.synchronize()
+    for r in res:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            outs.append(call(A, w, group, residual=r))
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for st, gr in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for o, r in zip(outs, want):
+            assert torch.equal(o, r)
+
+
+def test_linear_layers_use_the_epilogue(dev, monkeypatch):
+    """bind.linear_* with an activation or a residual: the kernels when they are switched on, the
+    stock path otherwise, the same values within fp16's rounding."""
+    from cuda_tempiler_b200 import bind
+    A = rand(5, 8, 512, seed=12)
+    bias, res = rand(272, seed=13), rand(5, 8, 272, seed=14)
+    for kind, group in (("fp16", 0), ("int8", 0), ("uint8", 128)):
+        w = weights(kind, 272, 512, group)
+        ys = []
+        for on in ("1", "0"):
+            monkeypatch.setenv("TEMPO_KERNELS", on)
+            bind.route_counts(reset=True)
+            if kind == "fp16":
+                y = bind.linear_fp16(A, w[0], bias, activation="gelu", residual=res)
+            else:
+                y = bind.linear_w8a16(A, *w, group, bias, activation="gelu", residual=res)
+            assert bind.route_counts()["tempo"] == int(on)
+            ys.append(y)
+        check(ys[0].reshape(40, 272), A.reshape(40, 512), w, group, bias, "gelu",
+              res.reshape(40, 272))
+        # the stock path rounds the weight, the product, the bias sum, the activation and the sum
+        assert torch.allclose(ys[0].float(), ys[1].float(), rtol=0, atol=2.0 ** -6)
+
+
+def test_refusals(dev):
+    from cuda_tempiler_b200 import ops
+    A, B = rand(8, 64), rand(48, 64)
+    W, s, z = weights("uint8", 48, 64, 64)
+    with pytest.raises(ValueError, match="activation"):
+        ops.gemm_fp16_epilogue(A, B, activation="tanh")
+    with pytest.raises(ValueError, match="bias"):
+        ops.gemm_fp16_epilogue(A, B, bias=rand(47))
+    with pytest.raises(ValueError, match="bias"):
+        ops.gemm_fp16_epilogue(A, B, bias=rand(48).float())
+    with pytest.raises(ValueError, match="bias"):
+        ops.gemm_fp16_epilogue(A, B, bias=rand(96)[::2])
+    with pytest.raises(ValueError, match="residual"):
+        ops.gemm_fp16_epilogue(A, B, residual=rand(8, 64))
+    with pytest.raises(ValueError, match="residual"):
+        ops.gemm_fp16_epilogue(A, B, residual=rand(48, 8).t())
+    with pytest.raises(ValueError, match="residual"):
+        ops.gemm_fp16_epilogue(A, B, residual=rand(8, 48).cpu())
+    with pytest.raises(ValueError, match="K mismatch"):
+        ops.gemm_fp16_epilogue(A, rand(48, 72))
+    with pytest.raises(ValueError, match="out"):
+        ops.gemm_fp16_epilogue(A, B, out=rand(8, 56))
+    with pytest.raises(ValueError, match="scale"):
+        ops.gemm_w8a16_epilogue(A, W, s.float(), z, 64)
+    with pytest.raises(ValueError, match="zero"):
+        ops.gemm_w8a16_epilogue(A, W, s, z[:, :40], 64)
+    with pytest.raises(ValueError, match="group"):
+        ops.gemm_w8a16_epilogue(A, W, s, None, 64)
+    buf = rand(10, 64)
+    with pytest.raises(ValueError, match="overlaps A"):
+        ops.gemm_fp16_epilogue(buf[:8], rand(64, 64), out=buf[2:])
+    with pytest.raises(ValueError, match="overlaps residual"):
+        ops.gemm_fp16_epilogue(A, rand(64, 64), residual=buf[:8], out=buf[1:9])
+    flat = rand(8 * 48 + 8)
+    with pytest.raises(ops.NotCovered):  # residual not 16-byte aligned
+        ops.gemm_fp16_epilogue(A, B, residual=flat[1:8 * 48 + 1].view(8, 48))
+    with pytest.raises(ops.NotCovered):
+        ops.gemm_fp16_epilogue(A, B, bias=rand(56)[1:49])
+    with pytest.raises(ops.NotCovered):
+        ops.gemm_fp16_epilogue(A, rand(44, 64))
+    with pytest.raises(ops.NotCovered):
+        ops.gemm_fp16_epilogue(A[:0], B)
