@@ -14,6 +14,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -21,6 +22,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 SHIPPED = PKG / "kernels" / "shipped"
+SKELETON = PKG / "tempo" / "plugins" / "sm100" / "skeletons" / "gemm_sm100"
 LIB = PKG / "libtempo_sm100.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -33,7 +35,8 @@ def nvcc() -> str:
 
 
 def sources() -> list:
-    return (sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh"))
+    return (sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+            + sorted(SKELETON.glob("*.cuh"))
             + sorted(SHIPPED.glob("*/sm_100a/*.cuh")) + sorted(SHIPPED.glob("*/sm_100a/*.cu"))
             + sorted(SHIPPED.glob("*/sm_100a/*.inc")) + [INCLUDE / "tempo_sm100.h"])
 
@@ -49,18 +52,29 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile every .cu under csrc/ into one shared library (no-op when up to date)."""
     if not force and not stale():
         return LIB
-    cmd = [
-        nvcc(), *ARCH_FLAGS, "-O3", "-std=c++17", "-lineinfo", "-Xptxas", "-v",
-        "-Xcompiler", "-fPIC", "-shared", f"-I{INCLUDE}", f"-I{CSRC}", f"-I{SHIPPED}",
-        "-o", str(LIB) + ".tmp", *[str(p) for p in sorted(CSRC.glob("*.cu"))],
-    ]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+    flags = [*ARCH_FLAGS, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC"]
+    with tempfile.TemporaryDirectory(dir=PKG, prefix="_build") as tmp:
+        # the translation units side by side, then one shared library
+        jobs = []
+        for src in sorted(CSRC.glob("*.cu")):
+            obj = os.path.join(tmp, src.stem + ".o")
+            cmd = [nvcc(), *flags, "-Xptxas", "-v", f"-I{INCLUDE}", f"-I{CSRC}", f"-I{SHIPPED}",
+                   "-c", "-o", obj, str(src)]
+            jobs.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE,
+                                               stderr=subprocess.PIPE, text=True)))
+        done = [(obj, p, *p.communicate()) for obj, p in jobs]
+        for _, p, out, err in done:
+            if p.returncode != 0:
+                raise RuntimeError("nvcc failed:\n" + out + err)
+        res = subprocess.run([nvcc(), *flags, "-shared", "-o", str(LIB) + ".tmp",
+                              *[obj for obj, *_ in done]], capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
     os.replace(str(LIB) + ".tmp", LIB)
-    (PKG / "libtempo_sm100.ptxas.log").write_text(res.stderr)
+    log = "".join(err for *_, err in done)
+    (PKG / "libtempo_sm100.ptxas.log").write_text(log)
     if verbose:
-        print(res.stderr)
+        print(log)
     return LIB
 
 

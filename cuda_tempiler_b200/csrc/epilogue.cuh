@@ -7,7 +7,7 @@
 //              (an int8 value is exact in fp16, its product with a scale is not).
 #pragma once
 
-#include "stream.cuh"
+#include "stream.h"
 
 namespace tempo_sm100 {
 
@@ -22,11 +22,11 @@ __global__ void __launch_bounds__(256)
   pdl_launch_dependents();
   const int n = (int)(i / per_row);
   const int k0 = (int)(i - (long long)n * per_row) * 16;
-  uint32_t h[8];
-  stream_unpack<kWInt8PerChannel>(ld_stream(W + (long long)n * ldw + k0), __half2{}, h);
+  __half2 h[8];
+  gemv_weights<kWInt8PerChannel>(ld_stream(W + (long long)n * ldw + k0), h, __half2{}, __half2{});
   uint4* o = reinterpret_cast<uint4*>(out + (long long)n * K + k0);
-  o[0] = make_uint4(h[0], h[1], h[2], h[3]);
-  o[1] = make_uint4(h[4], h[5], h[6], h[7]);
+  o[0] = *reinterpret_cast<const uint4*>(&h[0]);
+  o[1] = *reinterpret_cast<const uint4*>(&h[4]);
 }
 
 namespace {
@@ -67,7 +67,12 @@ cudaError_t run_tile_epi(const Problem& pr, const Hyper& h, cudaStream_t st) {
 }
 
 cudaError_t run_epilogue(const Problem& pr, cudaStream_t st) {
-  if (pr.M <= kStreamMaxM) return run_stream(pr, st);
+  if (pr.M <= kStreamMaxM)
+    return run_stream({static_cast<const __half*>(pr.A), static_cast<const uint8_t*>(pr.W),
+                       static_cast<const __half*>(pr.scale), static_cast<const uint8_t*>(pr.zero),
+                       static_cast<__half*>(pr.C), pr.epi, pr.M, pr.N, pr.K, pr.lda, pr.ldw,
+                       pr.ldc, pr.group > 0 ? pr.group : 1},
+                      pr.wkind, st);
   const size_t cap = pr.ws ? pr.ws_bytes : 0;
   tempo::gen::Choice c{};
   cudaError_t e;

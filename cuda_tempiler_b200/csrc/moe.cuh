@@ -9,12 +9,12 @@
 // tokens; everything else is small.  The products are those of stream.cuh: weights straight from
 // HBM into the registers of warp MMAs, fp32 sums, 8-bit weights as exact integers.
 //
-// The columns of every MMA are the tokens themselves (column m = token m): a token that did not
-// choose the expert is a column of zeros, which costs nothing beside the weight stream, and
-// k_moe_down can keep one fp32 sum per (n, token) in registers over all experts: no atomics, no
-// partial outputs, the same order of sums on every run.  A column a token did not choose is left
-// out of its sum (not added as zero), so an infinite weight of one expert reaches only the tokens
-// that chose it.
+// A slot is an expert with at most 16 of its tokens (an expert with more has several slots; the
+// second one finds the weights in L2).  The columns of its MMAs are its tokens in ascending
+// order, so an expert that two tokens chose costs one MMA per 16 x 16 weights however many tokens
+// the call has.  k_moe_down keeps one fp32 sum per (warp, token, row) in shared memory over all
+// slots: no atomics, no partial outputs, the same order of sums on every run, and an infinite
+// weight of an expert reaches only the tokens that chose it.
 //
 // h is kept in fp32.  The down product needs fp16 operands, so each row of h is scaled by a
 // power of two (its largest value to [2^14, 2^15)) and split into fp16 high and low parts: 22
@@ -29,15 +29,17 @@ constexpr int kMoeMaxT = 32;
 constexpr int kMoeMaxK = 16;
 constexpr int kMoeMaxE = 512;
 constexpr int kMoeMaxRows = kMoeMaxT * kMoeMaxK;
-constexpr int kRouteCluster = 8;
+constexpr int kMoeCols = 16;  // tokens of a slot
+constexpr int kRouteCluster = 16;
+constexpr int kPlanThreads = 256;
 
 // What the router tells the two products (in the caller's workspace; every call writes it whole).
 struct MoePlan {
-  int n_slots;                      // experts reached by at least one token
+  int n_slots;                      // every slot has a token, so at most T * top_k
   int pad[3];
-  int expert[kMoeMaxE];             // slot -> expert, ascending
-  int base[kMoeMaxE];               // slot -> its first row
-  unsigned mask[kMoeMaxE];          // slot -> its tokens; row of token t: base + rank of bit t
+  int expert[kMoeMaxRows];          // slot -> expert, ascending
+  int base[kMoeMaxRows];            // slot -> its first row; column c is row base + c
+  unsigned mask[kMoeMaxRows];       // slot -> its tokens; column c is the c-th set bit
   float weight[kMoeMaxRows];        // row -> routing weight
   unsigned amax[kMoeMaxRows];       // row -> bits of max |h| (k_moe_gate_up)
 };
@@ -75,24 +77,29 @@ __device__ void moe_build_plan(MoePlan* plan, const int* ids, const float* w, in
     for (int e0 = 0; e0 < E; e0 += 32) {
       const int e = e0 + tid;
       const unsigned m = e < E ? emask[e] : 0u;
-      const unsigned act = __ballot_sync(0xffffffffu, m != 0u);
       const int c = __popc(m);
-      int incl = c;
+      // rows and slots of the experts before this one, in one scan (rows < 2^16)
+      const int mine = c | ((c + kMoeCols - 1) / kMoeCols) << 16;
+      int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if (tid >= o) incl += v;
       }
-      const int b = row + incl - c;
+      const int excl = incl - mine;
+      int b = row + (excl & 0xffff), s = slot + (excl >> 16);
       if (e < E) ebase[e] = b;
-      if (m) {
-        const int s = slot + __popc(act & ((1u << tid) - 1u));
+      for (unsigned left = m; left; ++s, b += kMoeCols) {
+        unsigned rest = left;
+        for (int i = 0; i < kMoeCols && rest; ++i) rest &= rest - 1u;
         plan->expert[s] = e;
         plan->base[s] = b;
-        plan->mask[s] = m;
+        plan->mask[s] = left & ~rest;
+        left = rest;
       }
-      slot += __popc(act);
-      row += __shfl_sync(0xffffffffu, incl, 31);
+      const int all = __shfl_sync(0xffffffffu, incl, 31);
+      slot += all >> 16;
+      row += all & 0xffff;
     }
     if (tid == 0) plan->n_slots = slot;
   }
@@ -127,38 +134,37 @@ __device__ void moe_topk(const float* logits, int E, int k, bool normalize, int*
   constexpr int P = kMoeMaxE / 32;
   const int lane = threadIdx.x & 31;
   unsigned key[P];
-  unsigned long long nan_any = 0;
+  bool nan_any = false;
   float mx = -INFINITY;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
+    if (32 * p >= E) break;
     const int e = lane + 32 * p;
     key[p] = 0u;
     if (e < E) {
       const float x = logits[e];
       key[p] = logit_key(x);
-      nan_any |= (x != x);
+      nan_any |= x != x;
       mx = fmaxf(mx, x);
     }
   }
-  const bool bad = __any_sync(0xffffffffu, nan_any != 0);
+  const bool bad = __any_sync(0xffffffffu, nan_any);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float total = 0.f;
   if (!normalize) {
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (lane + 32 * p < E) total += expf(logits[lane + 32 * p] - mx);
+    for (int e = lane; e < E; e += 32) total += expf(logits[e] - mx);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
   unsigned taken = 0u;
-  float mine = 0.f;  // lane j keeps the j-th choice
-  int mine_id = 0;
+  int mine_id = 0;  // lane j keeps the j-th choice
   for (int j = 0; j < k; ++j) {
     unsigned best = 0u;
     int bp = -1;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
+      if (32 * p >= E) break;
       if (lane + 32 * p < E && !((taken >> p) & 1u) && (bp < 0 || key[p] > best)) {
         best = key[p];
         bp = p;
@@ -168,11 +174,9 @@ __device__ void moe_topk(const float* logits, int E, int k, bool normalize, int*
     const unsigned cand = (bp >= 0 && best == top) ? (unsigned)(lane + 32 * bp) : 0xffffffffu;
     const unsigned e = __reduce_min_sync(0xffffffffu, cand);
     if ((e & 31u) == (unsigned)lane) taken |= 1u << (e >> 5);
-    if (lane == j) {
-      mine_id = (int)e;
-      mine = expf(logits[e] - mx);
-    }
+    if (lane == j) mine_id = (int)e;
   }
+  const float mine = lane < k ? expf(logits[mine_id] - mx) : 0.f;
   if (normalize) {
     total = mine;
 #pragma unroll
@@ -184,131 +188,134 @@ __device__ void moe_topk(const float* logits, int E, int k, bool normalize, int*
   }
 }
 
-// One cluster of 8 CTAs routes 32 tokens: CTA r multiplies them with the experts
-// [E r / 8, E (r + 1) / 8) (its 8 warps split H), hands each token's logits to the CTA that owns
-// the token (t % 8) through distributed shared memory, and picks the top-k of its own tokens.
-// With a plan wanted (one cluster, T <= 32) CTA 0 collects the choices and builds it.
-// Each step's sum starts at zero and is added in fp32: a tensor core truncates what it adds to a
-// large accumulator, which over a long K is visible in fp32 weights.
+struct RouteArgs {
+  const __half* x;
+  long long ldx;
+  const __half* wr;
+  long long ldw;
+  const __half* bias;
+  int T, E, H, k, normalize;
+  int* ids;
+  float* weights;
+  MoePlan* plan;
+};
+
+// The experts [lo, hi) times the tokens [t0, t0 + nt), 16 experts at a time.
 template <int MG>
-__global__ void __launch_bounds__(kStreamThreads)
-    k_moe_route(const __half* __restrict__ x, long long ldx, const __half* __restrict__ wr,
-                long long ldw, const __half* __restrict__ bias, int T, int E, int H, int k,
-                int normalize, int* __restrict__ ids, float* __restrict__ weights,
-                MoePlan* plan) {
-  using S = StreamStep<kWFp16>;
-  constexpr int U = 4;
-  constexpr int TOK = MG * 8;                    // tokens of a cluster
-  constexpr int OWN = (TOK + kRouteCluster - 1) / kRouteCluster;
-  __shared__ float4 red[kStreamWarps][MG][32];
-  __shared__ float logits[OWN][kMoeMaxE];        // of this CTA's tokens
-  __shared__ int s_ids[kMoeMaxRows];             // CTA 0: every token's choices
-  __shared__ float s_w[kMoeMaxRows];
-  __shared__ unsigned emask[kMoeMaxE];
-  __shared__ int ebase[kMoeMaxE];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, t = lane & 3;
+struct RouteJob {
+  using St = StreamStep<kWFp16>;
+  using F = StreamFifo<kWFp16, MG, 1, 1>;
+  static constexpr bool ROTATE = false;  // equal router rows have equal logits
+  const RouteArgs& a;
+  int lo, hi, t0, nt, lane;
+  float* logits;  // [tokens this CTA owns][kMoeMaxE], the same place in every CTA of the cluster
+  struct Piece {
+    int n0;
+    const __half* w;
+  };
+  __device__ __forceinline__ bool at(Piece& p, int n0) const {
+    p.n0 = n0;
+    p.w = a.wr + (n0 + (lane >> 2)) * a.ldw + 8 * (lane & 3);
+    return n0 < hi;
+  }
+  __device__ __forceinline__ bool first(Piece& p) const { return at(p, lo); }
+  __device__ __forceinline__ bool next(Piece& p) const { return at(p, p.n0 + 16); }
+  __device__ __forceinline__ void copy(const Piece& p, int step, uint32_t stage) const {
+    const int g = lane >> 2, kw = step * St::STEP;
+    const bool ok = kw + 8 * (lane & 3) < a.H;
+    if (p.n0 + g < hi) cp_async16(stage + lane * 16, p.w + kw, ok);
+    if (p.n0 + g + 8 < hi) cp_async16(stage + 512 + lane * 16, p.w + 8 * a.ldw + kw, ok);
+#pragma unroll
+    for (int mg = 0; mg < MG; ++mg) {
+      const int m = mg * 8 + g;
+      if (m < nt)
+        cp_async16(stage + F::B_OFF + mg * 512 + lane * 16,
+                   a.x + (long long)(t0 + m) * a.ldx + kw + 8 * (lane & 3), ok);
+    }
+  }
+  __device__ __forceinline__ unsigned use_cols(const Piece&) const {
+    unsigned c = 0;
+#pragma unroll
+    for (int mg = 0; mg < MG; ++mg) c |= (mg * 8 + (lane >> 2) < nt ? 1u : 0u) << mg;
+    return c;
+  }
+  __device__ __forceinline__ unsigned live(const Piece&) const {
+    return (1u << ((nt + 7) / 8)) - 1u;
+  }
+  __device__ __forceinline__ void z_rows(const Piece&, int (&r)[1]) const { r[0] = 0; }
+  __device__ __forceinline__ void finish(const Piece& p, int, int mg, float4 v) const {
+    const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = p.n0 + (lane >> 2) + (j >= 2 ? 8 : 0);
+      const int m = mg * 8 + 2 * (lane & 3) + (j & 1);
+      if (e >= hi || m >= nt) continue;
+      const float z = o[j] + (a.bias ? __half2float(__ldg(a.bias + e)) : 0.f);
+      // token m's logits go to the CTA that picks its experts
+      st_dsmem_f32(mapa_shared(smem_u32(logits + (m / kRouteCluster) * kMoeMaxE + e),
+                               m % kRouteCluster), z);
+    }
+  }
+};
+
+template <int MG>
+struct RouteCfg {
+  static constexpr int NW = 16;
+  static constexpr int TOK = MG * 8;  // tokens of a cluster
+  static constexpr int OWN = (TOK + kRouteCluster - 1) / kRouteCluster;
+  using F = StreamFifo<kWFp16, MG, 1, 1>;
+  static constexpr int RED = 8 * MG * 512;
+  static constexpr int REST = OWN * kMoeMaxE * 4 + 2 * kMoeMaxRows * 4 + 2 * kMoeMaxE * 4;
+  static constexpr int S = F::depth((kMaxDynSmem - RED - REST) / NW);
+  static constexpr int FIFO = NW * S * F::STAGE;
+  static constexpr int SMEM = FIFO + RED + REST;
+};
+
+// One cluster of 16 CTAs routes 8 or 32 tokens: CTA r multiplies them with the experts
+// [E r / 16, E (r + 1) / 16) -- its share of the router's weights is in flight at once -- hands
+// each token's logits to the CTA that owns the token (t % 16) through distributed shared memory,
+// and picks the top-k of its own tokens, a warp each.  With a plan wanted (one cluster, T <= 32)
+// CTA 0 collects the choices and builds it.
+template <int MG>
+__global__ void __launch_bounds__(32 * RouteCfg<MG>::NW, 1) k_moe_route(const RouteArgs a) {
+  using C = RouteCfg<MG>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* logits = reinterpret_cast<float*>(smem + C::FIFO + C::RED);
+  int* s_ids = reinterpret_cast<int*>(logits + C::OWN * kMoeMaxE);  // CTA 0: everyone's choices
+  float* s_w = reinterpret_cast<float*>(s_ids + kMoeMaxRows);
+  unsigned* emask = reinterpret_cast<unsigned*>(s_w + kMoeMaxRows);
+  int* ebase = reinterpret_cast<int*>(emask + kMoeMaxE);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = (int)cluster_ctarank();
-  const int t0 = (blockIdx.x / kRouteCluster) * TOK;
-  const int nt = min(TOK, T - t0);
+  const int t0 = (blockIdx.x / kRouteCluster) * C::TOK;
+  const int nt = min(C::TOK, a.T - t0);
+  cluster_sync();  // every CTA of the cluster runs before its shared memory is written
   pdl_wait();
   pdl_launch_dependents();
-  cluster_sync();  // every CTA of the cluster runs before its shared memory is written
-  const int lo = E * rank / kRouteCluster, hi = E * (rank + 1) / kRouteCluster;
-  const int nsteps = (H + S::STEP - 1) / S::STEP;
-  for (int n0 = lo; n0 < hi; n0 += 16) {
-    float acc[MG][4] = {};
-    StreamStage<kWFp16, MG, 1> st[U];
-    auto load_b = [&](int step, int mg, uint32_t (&b)[S::NB]) {
-      const int k0 = step * S::STEP + t * S::KC;
-      const int m = mg * 8 + g;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (k0 < H && m < nt)
-        v = __ldg(reinterpret_cast<const uint4*>(x + (long long)(t0 + m) * ldx + k0));
-      b[0] = v.x;
-      b[1] = v.y;
-      b[2] = v.z;
-      b[3] = v.w;
-    };
-    auto load = [&](StreamStage<kWFp16, MG, 1>& s, int step) {
-      const int k0 = step * S::STEP + t * S::KC;
-      const bool ok = step < nsteps && k0 < H;
-      const int ra = n0 + g, rb = ra + 8;
-      s.xa[0] = s.xb[0] = make_uint4(0u, 0u, 0u, 0u);
-      if (ok && ra < hi) s.xa[0] = __ldg(reinterpret_cast<const uint4*>(wr + ra * ldw + k0));
-      if (ok && rb < hi) s.xb[0] = __ldg(reinterpret_cast<const uint4*>(wr + rb * ldw + k0));
-      if constexpr (kStreamPreB<kWFp16, MG>) {
-#pragma unroll
-        for (int mg = 0; mg < MG; ++mg) load_b(step, mg, s.b[mg]);
-      }
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u) load(st[u], warp + u * kStreamWarps);
-    for (int step = warp; step < nsteps;) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (step < nsteps) {
-          float d[1][MG][4] = {};
-          stream_mma<kWFp16, MG, 1>(
-              st[u], d, [&](int mg, uint32_t(&b)[S::NB]) { load_b(step, mg, b); },
-              [](int) { return true; });
-#pragma unroll
-          for (int mg = 0; mg < MG; ++mg)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[mg][j] += d[0][mg][j];
-          load(st[u], step + U * kStreamWarps);
-        }
-        step += kStreamWarps;
-      }
-    }
-#pragma unroll
-    for (int mg = 0; mg < MG; ++mg)
-      red[warp][mg][lane] = make_float4(acc[mg][0], acc[mg][1], acc[mg][2], acc[mg][3]);
-    __syncthreads();
-    for (int i = tid; i < MG * 32; i += kStreamThreads) {
-      const int l = i & 31, mg = i >> 5;
-      float4 v = red[0][mg][l];
-#pragma unroll
-      for (int w = 1; w < kStreamWarps; ++w) {
-        const float4 a = red[w][mg][l];
-        v.x += a.x;
-        v.y += a.y;
-        v.z += a.z;
-        v.w += a.w;
-      }
-      const float o[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = n0 + (l >> 2) + (j >= 2 ? 8 : 0);
-        const int m = mg * 8 + 2 * (l & 3) + (j & 1);
-        if (e >= hi || m >= nt) continue;
-        const float z = o[j] + (bias ? __half2float(__ldg(bias + e)) : 0.f);
-        st_dsmem_f32(mapa_shared(smem_u32(&logits[m / kRouteCluster][e]), m % kRouteCluster), z);
-      }
-    }
-    __syncthreads();
-  }
+  RouteJob<MG> job{a, a.E * rank / kRouteCluster, a.E * (rank + 1) / kRouteCluster, t0, nt, lane,
+                   logits};
+  stream_run<kWFp16, MG, 1, 1, C::NW, C::S, true>(
+      job, smem, reinterpret_cast<float4*>(smem + C::FIFO),
+      (a.H + StreamStep<kWFp16>::STEP - 1) / StreamStep<kWFp16>::STEP);
   cluster_sync();
-  for (int q = warp; q < OWN; q += kStreamWarps) {
+  for (int q = warp; q < C::OWN; q += C::NW) {
     const int m = q * kRouteCluster + rank;
     if (m >= nt) continue;
-    int* id = ids + (long long)(t0 + m) * k;
-    float* w = weights + (long long)(t0 + m) * k;
-    moe_topk(logits[q], E, k, normalize != 0, id, w);
-    __syncwarp();
-    if (plan && lane < k) {
-      // lane < k wrote these two itself
-      st_dsmem_f32(mapa_shared(smem_u32(&s_ids[m * k + lane]), 0), __int_as_float(id[lane]));
-      st_dsmem_f32(mapa_shared(smem_u32(&s_w[m * k + lane]), 0), w[lane]);
+    int* id = a.ids + (long long)(t0 + m) * a.k;
+    float* w = a.weights + (long long)(t0 + m) * a.k;
+    moe_topk(logits + q * kMoeMaxE, a.E, a.k, a.normalize != 0, id, w);
+    if (a.plan && lane < a.k) {  // this lane wrote these two itself
+      st_dsmem_f32(mapa_shared(smem_u32(s_ids + m * a.k + lane), 0), __int_as_float(id[lane]));
+      st_dsmem_f32(mapa_shared(smem_u32(s_w + m * a.k + lane), 0), w[lane]);
     }
   }
-  if (!plan) return;
+  if (!a.plan) return;
   cluster_sync();
-  if (rank == 0) moe_build_plan(plan, s_ids, s_w, T, k, E, emask, ebase);
+  if (rank == 0) moe_build_plan(a.plan, s_ids, s_w, a.T, a.k, a.E, emask, ebase);
 }
 
 // The plan of a routing the caller brings.
-__global__ void __launch_bounds__(kStreamThreads)
+__global__ void __launch_bounds__(kPlanThreads)
     k_moe_plan(const int* __restrict__ ids, const float* __restrict__ weights, int T, int k, int E,
                MoePlan* plan) {
   __shared__ int s_ids[kMoeMaxRows];
@@ -330,338 +337,440 @@ __device__ __forceinline__ int gate_row(int c, int block) {
   return block ? (c / block) * 2 * block + c % block : c;
 }
 
-// A row tile is 8 columns of h: MMA rows 0-7 are their gate rows, rows 8-15 their up rows, so
-// silu(gate) * up needs no exchange.  CTA b of G owns the tiles [n b / G, n (b + 1) / G) of the
-// n = n_slots * I / 8 tiles in slot order, taken in pieces of at most RT tiles of one slot.
-template <int WQ, int MG, int RT>
-__global__ void __launch_bounds__(kStreamThreads, 2) k_moe_gate_up(const MoeArgs a) {
-  using S = StreamStep<WQ>;
-  constexpr int U = stream_depth<WQ, MG, RT>();
-  __shared__ float4 red[kStreamWarps][RT][MG][32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  pdl_wait();
-  pdl_launch_dependents();
-  const MoePlan& plan = *a.plan;
-  const int per_slot = a.I / 8;
-  const long long n_tiles = (long long)plan.n_slots * per_slot;
-  const long long lo = n_tiles * blockIdx.x / gridDim.x;
-  const long long hi = n_tiles * (blockIdx.x + 1) / gridDim.x;
-  const int nsteps = (a.H + S::STEP - 1) / S::STEP;
-  const int up = a.gu_block ? a.gu_block : a.I;
-  const int groups = WQ == kWUint8Group ? a.H / a.group : 0;
-  for (long long pos = lo; pos < hi;) {
-    const int slot = (int)(pos / per_slot);
-    const int c_tile = (int)(pos - (long long)slot * per_slot);
-    const int left = (int)min((long long)(per_slot - c_tile), hi - pos);
-    const int np = (left + RT - 1) / RT;
-    const int cnt = (left + np - 1) / np;  // tiles of this piece (<= RT)
-    pos += cnt;
-    const int e = plan.expert[slot];
-    const unsigned mask = plan.mask[slot];
-    const int base = plan.base[slot];
-    const uint8_t* W = a.wgu + (long long)e * 2 * a.I * a.H * S::ESZ;
-    const __half* sc = WQ == kWFp16 ? nullptr
-                       : a.sgu + (long long)e * 2 * a.I * (WQ == kWUint8Group ? groups : 1);
-    const uint8_t* zp = WQ == kWUint8Group ? a.zgu + (long long)e * 2 * a.I * groups : nullptr;
-    float acc[RT][MG][4] = {};
-    StreamStage<WQ, MG, RT> st[U];
-    auto load_b = [&](int step, int mg, uint32_t (&b)[S::NB]) {
-      const int k0 = step * S::STEP + t * S::KC;
-      const int m = mg * 8 + g;
-#pragma unroll
-      for (int q = 0; q < S::KC / 8; ++q) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (k0 < a.H && ((mask >> m) & 1u))
-          v = __ldg(reinterpret_cast<const uint4*>(a.x + m * a.ldx + k0) + q);
-        b[4 * q] = v.x;
-        b[4 * q + 1] = v.y;
-        b[4 * q + 2] = v.z;
-        b[4 * q + 3] = v.w;
-      }
-    };
-    auto load = [&](StreamStage<WQ, MG, RT>& s, int step) {
-      const int k0 = step * S::STEP + t * S::KC;
-      const bool ok = step < nsteps && k0 < a.H;
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const int ra = gate_row((c_tile + rt) * 8 + g, a.gu_block), rb = ra + up;
-        const bool on = ok && rt < cnt;
-        s.xa[rt] = s.xb[rt] = make_uint4(0u, 0u, 0u, 0u);
-        if (on) {
-          s.xa[rt] = ld_stream(W + ((long long)ra * a.H + k0) * S::ESZ);
-          s.xb[rt] = ld_stream(W + ((long long)rb * a.H + k0) * S::ESZ);
-        }
-        if (WQ == kWUint8Group) {
-          s.s[rt] = 0;
-          s.z[rt] = 0;
-          if (on) {  // lane % 16 < 8: a gate row, else an up row
-            const int r = gate_row((c_tile + rt) * 8 + (lane & 7), a.gu_block) +
-                          ((lane & 8) ? up : 0);
-            const long long gi = (long long)(k0 / a.group) * 2 * a.I + r;
-            s.s[rt] = __ldg(reinterpret_cast<const unsigned short*>(sc) + gi);
-            s.z[rt] = __ldg(zp + gi);
-          }
-        }
-      }
-      if constexpr (kStreamPreB<WQ, MG>) {
-#pragma unroll
-        for (int mg = 0; mg < MG; ++mg) load_b(step, mg, s.b[mg]);
-      }
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u) load(st[u], warp + u * kStreamWarps);
-    for (int step = warp; step < nsteps;) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (step < nsteps) {
-          stream_mma<WQ, MG, RT>(
-              st[u], acc, [&](int mg, uint32_t(&b)[S::NB]) { load_b(step, mg, b); },
-              [&](int mg) { return ((mask >> (8 * mg)) & 0xffu) != 0u; });
-          load(st[u], step + U * kStreamWarps);
-        }
-        step += kStreamWarps;
-      }
+// The plan's slots in shared memory, for kernels that look them up as they go.
+struct SlotTable {
+  int* expert;
+  int* base;
+  unsigned* mask;
+  __device__ __forceinline__ SlotTable(uint8_t* smem, int rows)
+      : expert(reinterpret_cast<int*>(smem)), base(expert + rows),
+        mask(reinterpret_cast<unsigned*>(base + rows)) {}
+  __device__ __forceinline__ void load(const MoePlan& p, int n_slots) {
+    for (int i = threadIdx.x; i < n_slots; i += blockDim.x) {
+      expert[i] = p.expert[i];
+      base[i] = p.base[i];
+      mask[i] = p.mask[i];
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int mg = 0; mg < MG; ++mg)
-        red[warp][rt][mg][lane] =
-            make_float4(acc[rt][mg][0], acc[rt][mg][1], acc[rt][mg][2], acc[rt][mg][3]);
-    __syncthreads();
-    // RT * MG * 32 items; every warp runs whole (rt, mg) groups, so the shuffles are convergent
-    for (int i = tid; i < RT * MG * 32; i += kStreamThreads) {
-      const int mg = (i >> 5) % MG, rt = (i >> 5) / MG;
-      if (rt >= cnt) continue;
-      float4 v = red[0][rt][mg][lane];
-#pragma unroll
-      for (int w = 1; w < kStreamWarps; ++w) {
-        const float4 q = red[w][rt][mg][lane];
-        v.x += q.x;
-        v.y += q.y;
-        v.z += q.z;
-        v.w += q.w;
-      }
-      const int c = (c_tile + rt) * 8 + g;
-      float sg = 1.f, su = 1.f;
-      if (WQ == kWInt8PerChannel) {
-        const int ra = gate_row(c, a.gu_block);
-        sg = __half2float(__ldg(sc + ra));
-        su = __half2float(__ldg(sc + ra + up));
-      }
-      const float gt[2] = {v.x * sg, v.y * sg}, ut[2] = {v.z * su, v.w * su};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int m = mg * 8 + 2 * t + j;
-        const bool on = (mask >> m) & 1u;
-        const int row = base + __popc(mask & ((1u << m) - 1u));
-        float hv = 0.f;
-        if (on) {
-          hv = gt[j] / (1.f + expf(-gt[j])) * ut[j] * plan.weight[row];
-          a.h[(long long)row * a.I + c] = hv;
-        }
-        unsigned bits = __float_as_uint(fabsf(hv));
-        bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
-        bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 8));
-        bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 16));
-        if (on && g == 0) atomicMax(&a.plan->amax[row], bits);
-      }
-    }
-    __syncthreads();
   }
+};
+
+// Token of column c of a slot (the c-th set bit); -1 past its last.
+__device__ __forceinline__ int slot_token(unsigned mask, int c) {
+  for (int i = 0; i < c && mask; ++i) mask &= mask - 1u;
+  return __ffs((int)mask) - 1;
 }
 
-// 2^s that takes a largest value with these bits to [2^14, 2^15); 1 for zero, infinite and NaN.
+// A row tile is 8 columns of h: MMA rows 0-7 are their gate rows, rows 8-15 their up rows, so
+// silu(gate) * up needs no exchange.  CTA b of G owns the quads of columns [n b / G, n (b + 1) / G)
+// of the n = n_slots * I / 4 in slot order (whole tiles would be 6 or 7 for each CTA where one
+// token reaches 4 experts), taken in pieces of at most RT tiles of one slot, the last one partly
+// filled.
+template <int WQ, int MG, int RT>
+struct GateUpJob {
+  using St = StreamStep<WQ>;
+  using F = StreamFifo<WQ, MG, RT, St::NB / 4>;
+  static constexpr bool ROTATE = true;
+  const MoeArgs& a;
+  const SlotTable& tab;
+  long long lo, hi;
+  int lane, up, per_slot;
+  long long up_bytes;  // from a gate row to its up row
+  unsigned per_group;  // group_magic
+  struct Piece {
+    long long end;        // first quad after the piece
+    int slot, c0, c1;     // its columns
+    unsigned mask;
+    int tok[MG];          // token of this lane's column of each group, or -1
+    const uint8_t* w[RT];  // this lane's chunk of each tile's gate row at k = 0
+    const __half* x[MG];   // vector lane % 4 of the token of column lane / 4
+    long long z;           // group-wise: where the slot's scales and zero points start
+  };
+  __device__ __forceinline__ bool at(Piece& p, long long pos) const {
+    if (pos >= hi) return false;
+    p.slot = (int)(pos / per_slot);
+    const int q = (int)(pos - (long long)p.slot * per_slot);
+    const int left = (int)min((long long)(per_slot - q), hi - pos);
+    const int np = (left + 2 * RT - 1) / (2 * RT);
+    const int cnt = (left + np - 1) / np;
+    p.c0 = 4 * q;
+    p.c1 = 4 * (q + cnt);
+    p.end = pos + cnt;
+    p.mask = tab.mask[p.slot];
+    const long long e = tab.expert[p.slot];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      // past the piece's columns the last one's row (never copied)
+      const int c = min(p.c0 + rt * 8 + (lane >> 2), p.c1 - 1);
+      p.w[rt] = a.wgu + ((e * 2 * a.I + gate_row(c, a.gu_block)) * a.H + (lane & 3) * St::KC) * St::ESZ;
+    }
+#pragma unroll
+    for (int mg = 0; mg < MG; ++mg) {
+      p.tok[mg] = slot_token(p.mask, mg * 8 + (lane >> 2));
+      p.x[mg] = a.x + max(p.tok[mg], 0) * a.ldx + 8 * (lane & 3);
+    }
+    if (WQ == kWUint8Group) p.z = e * (a.H / a.group) * 2 * a.I;
+    return true;
+  }
+  __device__ __forceinline__ bool first(Piece& p) const { return at(p, lo); }
+  __device__ __forceinline__ bool next(Piece& p) const { return at(p, p.end); }
+  __device__ __forceinline__ void copy(const Piece& p, int step, uint32_t stage) const {
+    const int kw = step * St::STEP;
+    const bool ok = kw + (lane & 3) * St::KC < a.H;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int c = p.c0 + rt * 8;
+      if (c >= p.c1) break;  // columns past the piece are never stored
+      const uint8_t* src = p.w[rt] + kw * St::ESZ;
+      const uint32_t d = stage + rt * 1024 + lane * 16;
+      if (c + (lane >> 2) < p.c1) {
+        cp_async16(d, src, ok);
+        cp_async16(d + 512, src + up_bytes, ok);
+      }
+      if (WQ == kWUint8Group) {
+        // 8 gate and 8 up rows: lanes 0-7 two scales each, lanes 16-19 four zero points (columns
+        // come in quads, blocks of rows are multiples of 8)
+        const long long gi = p.z + (long long)step_group(step, per_group) * 2 * a.I;
+        const uint32_t z = stage + F::Z_OFF + rt * 128;
+        if (lane < 8) {
+          const int cc = c + 2 * (lane & 3);
+          if (cc < p.c1)
+            cp_async4(z + 4 * lane, a.sgu + gi + gate_row(cc, a.gu_block) + (lane < 4 ? 0 : up), true);
+        } else if (lane >= 16 && lane < 20) {
+          const int cc = c + 4 * (lane & 1);
+          if (cc < p.c1)
+            cp_async4(z + 64 + 4 * (lane - 16),
+                      a.zgu + gi + gate_row(cc, a.gu_block) + (lane < 18 ? 0 : up), true);
+        }
+      }
+    }
+#pragma unroll
+    for (int mg = 0; mg < MG; ++mg) {
+      if (p.tok[mg] >= 0) {
+#pragma unroll
+        for (int v = 0; v < St::NB / 4; ++v)
+          cp_async16(stage + F::B_OFF + b_vec<St::NB / 4>(mg, 4 * v + (lane & 3), lane >> 2),
+                     p.x[mg] + kw + 32 * v, kw + 32 * v + 8 * (lane & 3) < a.H);
+      }
+    }
+  }
+  __device__ __forceinline__ unsigned use_cols(const Piece& p) const {
+    unsigned c = 0;
+#pragma unroll
+    for (int mg = 0; mg < MG; ++mg) c |= (p.tok[mg] >= 0 ? 1u : 0u) << mg;
+    return c;
+  }
+  __device__ __forceinline__ unsigned live(const Piece& p) const {
+    return __popc(p.mask) > 8 ? 3u : 1u;
+  }
+  __device__ __forceinline__ void z_rows(const Piece&, int (&r)[RT]) const {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) r[rt] = 0;
+  }
+  __device__ __forceinline__ void finish(const Piece& p, int rt, int mg, float4 v) const {
+    const int n_cols = __popc(p.mask);
+    if (p.c0 + rt * 8 >= p.c1 || mg * 8 >= n_cols) return;  // warp-uniform
+    const int g = lane >> 2, t = lane & 3;
+    const int c = p.c0 + rt * 8 + g;
+    const bool in = c < p.c1;
+    float sg = 1.f, su = 1.f;
+    if (WQ == kWInt8PerChannel && in) {
+      const __half* sc = a.sgu + (long long)tab.expert[p.slot] * 2 * a.I + gate_row(c, a.gu_block);
+      sg = __half2float(__ldg(sc));
+      su = __half2float(__ldg(sc + up));
+    }
+    const float gt[2] = {v.x * sg, v.y * sg}, ut[2] = {v.z * su, v.w * su};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int col = mg * 8 + 2 * t + j;
+      const bool on = col < n_cols;
+      const int row = tab.base[p.slot] + col;
+      float hv = 0.f;
+      if (on && in) {
+        hv = gt[j] / (1.f + expf(-gt[j])) * ut[j] * a.plan->weight[row];
+        a.h[(long long)row * a.I + c] = hv;
+      }
+      unsigned bits = __float_as_uint(fabsf(hv));
+      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 4));
+      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 8));
+      bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 16));
+      if (on && g == 0) atomicMax(&a.plan->amax[row], bits);  // a maximum: any order
+    }
+  }
+};
+
+template <int WQ, int MG, int RT>
+struct GateUpCfg {
+  static constexpr int NW = GU_NW;
+  static constexpr int BV = StreamStep<WQ>::NB / 4;
+  using F = StreamFifo<WQ, MG, RT, BV>;
+  static constexpr int RED = 8 * RT * MG * 512;
+  static constexpr int S = F::depth((kMaxDynSmem - RED - kMoeMaxRows * 12) / NW);
+  static constexpr int FIFO = NW * S * F::STAGE;
+  static constexpr int SMEM = FIFO + RED;  // + the slot table
+  static_assert(SMEM + kMoeMaxRows * 12 <= kMaxDynSmem, "shared memory");
+};
+
+template <int WQ, int MG, int RT>
+__global__ void __launch_bounds__(32 * GateUpCfg<WQ, MG, RT>::NW, 1)
+    k_moe_gate_up(const MoeArgs a, int rows) {
+  using C = GateUpCfg<WQ, MG, RT>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  SlotTable tab(smem + C::SMEM, rows);
+  pdl_wait();
+  pdl_launch_dependents();
+  const int n_slots = a.plan->n_slots;
+  tab.load(*a.plan, n_slots);
+  __syncthreads();
+  const int per_slot = a.I / 4;
+  const long long n = (long long)n_slots * per_slot;
+  GateUpJob<WQ, MG, RT> job{a, tab, n * blockIdx.x / gridDim.x, n * (blockIdx.x + 1) / gridDim.x,
+                            (int)(threadIdx.x & 31), a.gu_block ? a.gu_block : a.I, per_slot,
+                            (long long)(a.gu_block ? a.gu_block : a.I) * a.H *
+                                StreamStep<WQ>::ESZ,
+                            group_magic<WQ>(a.group)};
+  stream_run<WQ, MG, RT, C::BV, C::NW, C::S>(
+      job, smem, reinterpret_cast<float4*>(smem + C::FIFO),
+      (a.H + StreamStep<WQ>::STEP - 1) / StreamStep<WQ>::STEP);
+}
+
+// s such that 2^s takes a largest value with these bits to [2^14, 2^15); 0 for zero.
+constexpr int kNotFinite = 127;
 __device__ __forceinline__ int pow2_shift(unsigned amax_bits) {
   const int ex = (int)(amax_bits >> 23);
-  if (ex == 0 || ex == 255) return 0;
+  if (ex == 255) return kNotFinite;
+  if (ex == 0) return 0;
   return max(-126, min(126, 127 + 14 - ex));
 }
 __device__ __forceinline__ float pow2f(int s) { return __int_as_float((127 + s) << 23); }
 
-// Rows of y are split like k_stream_linear's (CTA b: [H b / G, H (b + 1) / G)); a warp walks the
+// Rows of y are split like k_stream_linear's (CTA b: [H b / G, H (b + 1) / G)).  A warp walks the
 // steps of all slots as one sequence (warp w: steps w, w + 8, ...), so the weight stream does not
-// pause between experts.
+// pause between experts; at a slot's end it adds its sums to its own fp32 sums per token in shared
+// memory, which are added over the warps, in warp order, at the end.  The FIFO holds the fp32 h of
+// a slot's first 8 tokens; those of tokens 9-16, which few slots have, are read when used.
 template <int WQ, int MG, int RT>
-__global__ void __launch_bounds__(kStreamThreads, 2) k_moe_down(const MoeArgs a) {
-  using S = StreamStep<WQ>;
-  constexpr int U = RT == 1 ? (MG == 4 ? 3 : 4) : (MG == 4 && WQ ? 1 : 2);
-  __shared__ float4 red[kStreamWarps][RT][MG][32];
-  __shared__ int s_expert[kMoeMaxE], s_base[kMoeMaxE];
-  __shared__ unsigned s_mask[kMoeMaxE];
-  __shared__ signed char s_shift[kMoeMaxRows];
+struct DownCfg {
+  using St = StreamStep<WQ>;
+  static constexpr int NW = MG == 1 ? DN_NW : DN_NW2;  // the sums of 32 tokens leave room for 8 warps
+  static constexpr int MAX_T = MG == 1 ? 8 : kMoeMaxT;
+  static constexpr int HV = St::KC / 4;  // 16-byte vectors of an fp32 chunk
+  using F = StreamFifo<WQ, 1, RT, HV>;
+  static constexpr int YROW = RT * 16 + 8;  // floats per token (padded: 4 tokens, 4 bank groups)
+  __host__ __device__ static constexpr int y_bytes(int T) { return NW * T * YROW * 4; }
+  static constexpr int TABLE = MAX_T * kMoeMaxK * 13 + 16;
+  static constexpr int S = F::depth((kMaxDynSmem - y_bytes(MAX_T) - TABLE) / NW);
+  static constexpr int FIFO = NW * S * F::STAGE;
+  __host__ __device__ static constexpr int smem(int T, int rows) {
+    return FIFO + y_bytes(T) + rows * 13 + 16;
+  }
+  static_assert(FIFO + y_bytes(MAX_T) + TABLE <= kMaxDynSmem, "shared memory");
+};
+
+template <int WQ, int MG, int RT>
+__global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
+    k_moe_down(const MoeArgs a, int rows) {
+  using C = DownCfg<WQ, MG, RT>;
+  using St = StreamStep<WQ>;
+  using F = typename C::F;
+  constexpr int S = C::S, HV = C::HV, NW = C::NW;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* y_all = reinterpret_cast<float*>(smem + C::FIFO);
+  SlotTable tab(smem + C::FIFO + C::y_bytes(a.T), rows);
+  signed char* shift = reinterpret_cast<signed char*>(tab.mask + rows);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  pdl_wait();
-  pdl_launch_dependents();
+  // The plan may be read before the wait: k_moe_gate_up lets this grid start only after its own
+  // wait, when the router (and all before it) had finished.  So the first steps' weights are
+  // fetched here, under the rest of k_moe_gate_up; only h and its largest values need the wait.
   const int n_slots = a.plan->n_slots;
-  for (int i = tid; i < n_slots; i += kStreamThreads) {
-    s_expert[i] = a.plan->expert[i];
-    s_base[i] = a.plan->base[i];
-    s_mask[i] = a.plan->mask[i];
-  }
-  __syncthreads();
-  const int n_rows =
-      n_slots ? s_base[n_slots - 1] + __popc(s_mask[n_slots - 1]) : 0;
-  for (int i = tid; i < n_rows; i += kStreamThreads)
-    s_shift[i] = (signed char)pow2_shift(a.plan->amax[i]);
+  tab.load(*a.plan, n_slots);
   __syncthreads();
   const int lo = (int)((long long)a.H * blockIdx.x / gridDim.x);
   const int hi = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x);
-  const int nsteps = (a.I + S::STEP - 1) / S::STEP;
-  const int total = n_slots * nsteps;
-  const int groups = WQ == kWUint8Group ? a.I / a.group : 1;
+  const int nsteps = (a.I + St::STEP - 1) / St::STEP;
   const int npieces = (hi - lo + 16 * RT - 1) / (16 * RT);
-  struct Stage {
-    uint4 xa[RT], xb[RT];
-    unsigned short s[RT];
-    uint8_t z[RT];
+  float* y = y_all + warp * a.T * C::YROW;
+  const uint32_t fifo = smem_u32(smem) + warp * S * F::STAGE;
+  // the warp's next step in the sequence of all slots' steps
+  const int rot = (int)((long long)nsteps * blockIdx.x / gridDim.x);
+  auto advance = [&](int& slot, int& step) {
+    step += NW;
+    while (step >= nsteps) {
+      step -= nsteps;
+      ++slot;
+    }
+  };
+  auto k_of = [&](int step) {  // this lane's first k of a step (rotated as in stream_run)
+    const int s = step + rot;
+    return (s < nsteps ? s : s - nsteps) * St::STEP;
   };
   for (int pc = 0; pc < npieces; ++pc) {
     const int n0 = lo + (hi - lo) * pc / npieces;
     const int n1 = lo + (hi - lo) * (pc + 1) / npieces;
-    float acc[RT][MG][4] = {};
-    Stage st[U];
-    auto load = [&](Stage& s, int fs) {
-      const int slot = fs / nsteps;
-      const int k0 = (fs - slot * nsteps) * S::STEP + t * S::KC;
-      const bool ok = fs < total && k0 < a.I;
-      const int e = fs < total ? s_expert[slot] : 0;
-      const uint8_t* W = a.wd + (long long)e * a.H * a.I * S::ESZ;
-      const long long gi = WQ == kWUint8Group
-                               ? ((long long)e * groups + k0 / a.group) * a.H
-                               : (long long)e * a.H;
+    for (int i = lane; i < a.T * C::YROW; i += 32) y[i] = 0.f;
+    // rows this lane's copies belong to, and where they start in an expert's matrix
+    const long long row_bytes = (long long)a.I * St::ESZ;
+    const uint8_t* w0 = a.wd + (n0 + g) * row_bytes + t * 16;
+    const unsigned magic = group_magic<WQ>(a.group);
+    int lslot = 0, lstep = warp, lfifo = 0;
+    while (lstep >= nsteps) {
+      lstep -= nsteps;
+      ++lslot;
+    }
+    int uslot = lslot, ustep = lstep;
+    auto issue = [&](bool weights, bool hidden) {
+      if (lslot < n_slots) {
+        const int step = lstep + rot < nsteps ? lstep + rot : lstep + rot - nsteps;
+        const int kw = step * St::STEP;
+        const int e = tab.expert[lslot];
+        const uint32_t stage = fifo + lfifo * F::STAGE;
+        if (weights) {
+          const bool ok = kw + t * St::KC < a.I;
+          const uint8_t* src = w0 + ((long long)e * a.H * row_bytes + kw * St::ESZ);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const int ra = n0 + rt * 16 + g, rb = ra + 8;
-        s.xa[rt] = s.xb[rt] = make_uint4(0u, 0u, 0u, 0u);
-        if (ok && ra < n1) s.xa[rt] = ld_stream(W + ((long long)ra * a.I + k0) * S::ESZ);
-        if (ok && rb < n1) s.xb[rt] = ld_stream(W + ((long long)rb * a.I + k0) * S::ESZ);
-        s.s[rt] = 0;
-        s.z[rt] = 0;
-        if (WQ) {  // scale (and zero point) of row lane % 16; k0 >= I only in int8's last step
-          const int r = n0 + rt * 16 + (lane & 15);
-          if (fs < total && r < n1) {
-            s.s[rt] = __ldg(reinterpret_cast<const unsigned short*>(a.sd) + gi + r);
-            if (WQ == kWUint8Group) s.z[rt] = __ldg(a.zd + gi + r);
+          for (int rt = 0; rt < RT; ++rt) {
+            const int ra = n0 + rt * 16 + g;
+            const uint32_t d = stage + rt * 1024 + lane * 16;
+            // rows past the piece are never stored
+            if (ra < n1) cp_async16(d, src + 2 * rt * 8 * row_bytes, ok);
+            if (ra + 8 < n1) cp_async16(d + 512, src + (2 * rt + 1) * 8 * row_bytes, ok);
+            if (WQ == kWUint8Group) {
+              const long long gi =
+                  ((long long)e * (a.I / a.group) + step_group(step, magic)) * a.H;
+              copy_group_row(stage + F::Z_OFF + rt * 128, a.sd + gi, a.zd + gi, n0 + rt * 16,
+                             a.H, lane, true);
+            }
           }
         }
-      }
-    };
-    auto use = [&](const Stage& s, int fs) {
-      const int slot = fs / nsteps;
-      const int k0 = (fs - slot * nsteps) * S::STEP + t * S::KC;
-      const unsigned mask = s_mask[slot];
-      const int base = s_base[slot];
-      uint32_t ha[RT][8], hb[RT][8];
-      float fa[RT], fb[RT];
+        if (hidden && g < __popc(tab.mask[lslot])) {
+          const float* h = a.h + (long long)(tab.base[lslot] + g) * a.I + kw + 4 * t;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const unsigned sz = (unsigned)s.s[rt] << 16 | s.z[rt];
-        const unsigned za = WQ ? __shfl_sync(0xffffffffu, sz, g) : 0u;
-        const unsigned zb = WQ ? __shfl_sync(0xffffffffu, sz, g + 8) : 0u;
-        fa[rt] = WQ ? __half2float(__ushort_as_half((unsigned short)(za >> 16))) : 1.f;
-        fb[rt] = WQ ? __half2float(__ushort_as_half((unsigned short)(zb >> 16))) : 1.f;
-        stream_unpack<WQ>(s.xa[rt], zero_bias((uint8_t)za), ha[rt]);
-        stream_unpack<WQ>(s.xb[rt], zero_bias((uint8_t)zb), hb[rt]);
+          for (int v = 0; v < HV; ++v)
+            cp_async16(stage + F::B_OFF + b_vec<HV>(0, 4 * v + t, g), h + 16 * v,
+                       kw + 16 * v + 4 * t < a.I);
+        }
+        advance(lslot, lstep);
       }
+      if (hidden) cp_async_commit();
+      lfifo = lfifo + 1 == S ? 0 : lfifo + 1;
+    };
+    if (pc == 0) {
+      const int lslot0 = lslot, lstep0 = lstep;
+#pragma unroll 1
+      for (int i = 0; i < S - 1; ++i) issue(true, false);
+      lslot = lslot0;
+      lstep = lstep0;
+      lfifo = 0;
+      pdl_wait();
+      pdl_launch_dependents();
+      for (int i = tid; i < rows; i += 32 * NW)
+        shift[i] = (signed char)pow2_shift(a.plan->amax[i]);
+#pragma unroll 1
+      for (int i = 0; i < S - 1; ++i) issue(false, true);
+      __syncthreads();
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < S - 1; ++i) issue(true, true);
+    }
+    int ufifo = 0;
+    int z_row[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) z_row[rt] = n0 + rt * 16;
+    while (uslot < n_slots) {
+      const int slot = uslot;
+      const unsigned mask = tab.mask[slot];
+      const int base = tab.base[slot], n_cols = __popc(mask);
+      float up2[MG];  // 2^s of this lane's columns
+      bool fin[MG];   // whether the row of h is finite: if not its low parts (inf - inf) are left out
 #pragma unroll
       for (int mg = 0; mg < MG; ++mg) {
-        if (((mask >> (8 * mg)) & 0xffu) == 0u) continue;  // warp-uniform
-        const int m = mg * 8 + g;
-        uint32_t bh[S::NB], bl[S::NB];
-        if (k0 < a.I && ((mask >> m) & 1u)) {
-          const int row = base + __popc(mask & ((1u << m) - 1u));
-          const float f = pow2f(s_shift[row]);
-          const float4* hp = reinterpret_cast<const float4*>(a.h + (long long)row * a.I + k0);
+        const int sh = mg * 8 + g < n_cols ? shift[base + mg * 8 + g] : 0;
+        fin[mg] = sh != kNotFinite;
+        up2[mg] = fin[mg] ? pow2f(sh) : 1.f;
+      }
+      float acc[RT][MG][4] = {};
+      while (uslot == slot) {
+        cp_async_wait<S - 2>();
+        __syncwarp();
+        issue(true, true);
+        const uint32_t stage = fifo + ufifo * F::STAGE;
+        StreamA<WQ, RT> w;
+        stream_read_weights<WQ, RT>(w, stage, F::Z_OFF, z_row, lane);
 #pragma unroll
-          for (int q = 0; q < S::KC / 4; ++q) {
-            const float4 v = hp[q];
-            const float s4[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+        for (int mg = 0; mg < MG; ++mg) {
+          if (mg * 8 >= n_cols) continue;  // warp-uniform
+          uint32_t bh[St::NB], bl[St::NB];
+          const bool on = mg * 8 + g < n_cols;
+#pragma unroll
+          for (int v = 0; v < HV; ++v) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (on) {
+              if (mg == 0) {
+                const uint4 q = lds16(stage + F::B_OFF + b_vec<HV>(0, HV * t + v, g));
+                x = make_float4(__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z),
+                                __uint_as_float(q.w));
+              } else {
+                const int k0 = k_of(ustep) + t * St::KC;
+                if (k0 < a.I)
+                  x = *reinterpret_cast<const float4*>(
+                      a.h + (long long)(base + mg * 8 + g) * a.I + k0 + 4 * v);
+              }
+            }
+            const float s4[4] = {x.x * up2[mg], x.y * up2[mg], x.z * up2[mg], x.w * up2[mg]};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const __half2 hi2 = __floats2half2_rn(s4[2 * i], s4[2 * i + 1]);
               const float2 back = __half22float2(hi2);
-              // an infinite high part has no low part (inf - inf is NaN)
-              const float l0 = isinf(back.x) ? 0.f : s4[2 * i] - back.x;
-              const float l1 = isinf(back.y) ? 0.f : s4[2 * i + 1] - back.y;
-              const __half2 lo2 = __floats2half2_rn(l0, l1);
-              bh[2 * q + i] = *reinterpret_cast<const uint32_t*>(&hi2);
-              bl[2 * q + i] = *reinterpret_cast<const uint32_t*>(&lo2);
+              const __half2 lo2 =
+                  __floats2half2_rn(s4[2 * i] - back.x, s4[2 * i + 1] - back.y);
+              bh[2 * v + i] = *reinterpret_cast<const uint32_t*>(&hi2);
+              bl[2 * v + i] = fin[mg] ? *reinterpret_cast<const uint32_t*>(&lo2) : 0u;
             }
           }
-        } else {
 #pragma unroll
-          for (int i = 0; i < S::NB; ++i) bh[i] = bl[i] = 0u;
+          for (int rt = 0; rt < RT; ++rt) {
+            stream_mma<WQ, RT>(w, rt, bh, acc[rt][mg]);
+            stream_mma<WQ, RT>(w, rt, bl, acc[rt][mg]);
+          }
         }
-        // this lane's two columns: their 2^-s, and whether the token chose the expert
-        const int m0 = mg * 8 + 2 * t;
-        const bool on0 = (mask >> m0) & 1u, on1 = (mask >> (m0 + 1)) & 1u;
-        const int r0 = base + __popc(mask & ((1u << m0) - 1u));
-        const float f0 = on0 ? pow2f(-s_shift[r0]) : 0.f;
-        const float f1 = on1 ? pow2f(-s_shift[r0 + (on0 ? 1 : 0)]) : 0.f;
+        ufifo = ufifo + 1 == S ? 0 : ufifo + 1;
+        advance(uslot, ustep);
+      }
+      // the slot's sums: undo the row's power of two, apply the channel's scale
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int mg = 0; mg < MG; ++mg) {
 #pragma unroll
-          for (int j = 0; j < S::NMMA; ++j) {
-            mma_16816(d, ha[rt][2 * j], hb[rt][2 * j], ha[rt][2 * j + 1], hb[rt][2 * j + 1],
-                      bh[2 * j], bh[2 * j + 1]);
-            mma_16816(d, ha[rt][2 * j], hb[rt][2 * j], ha[rt][2 * j + 1], hb[rt][2 * j + 1],
-                      bl[2 * j], bl[2 * j + 1]);
-          }
-          if (on0) {
-            acc[rt][mg][0] = fmaf(d[0], fa[rt] * f0, acc[rt][mg][0]);
-            acc[rt][mg][2] = fmaf(d[2], fb[rt] * f0, acc[rt][mg][2]);
-          }
-          if (on1) {
-            acc[rt][mg][1] = fmaf(d[1], fa[rt] * f1, acc[rt][mg][1]);
-            acc[rt][mg][3] = fmaf(d[3], fb[rt] * f1, acc[rt][mg][3]);
+        for (int j = 0; j < 2; ++j) {
+          const int col = mg * 8 + 2 * t + j;
+          if (col >= n_cols) continue;
+          float* yt = y + slot_token(mask, col) * C::YROW;
+          const int sh = shift[base + col];
+          const float f = sh != kNotFinite ? pow2f(-sh) : 1.f;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int r = rt * 16 + 8 * half + g;
+              float v = acc[rt][mg][2 * half + j] * f;
+              if (WQ == kWInt8PerChannel && n0 + r < n1)
+                v *= __half2float(__ldg(a.sd + (long long)tab.expert[slot] * a.H + n0 + r));
+              yt[r] += v;
+            }
           }
         }
       }
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u) load(st[u], warp + u * kStreamWarps);
-    for (int fs = warp; fs < total;) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (fs < total) {
-          use(st[u], fs);
-          load(st[u], fs + U * kStreamWarps);
-        }
-        fs += kStreamWarps;
-      }
+      __syncwarp();
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int mg = 0; mg < MG; ++mg)
-        red[warp][rt][mg][lane] =
-            make_float4(acc[rt][mg][0], acc[rt][mg][1], acc[rt][mg][2], acc[rt][mg][3]);
+    cp_async_wait<0>();
     __syncthreads();
-    for (int i = tid; i < RT * MG * 32; i += kStreamThreads) {
-      const int mg = (i >> 5) % MG, rt = (i >> 5) / MG;
-      float4 v = red[0][rt][mg][lane];
+    const int nr = n1 - n0;
+    for (int i = tid; i < a.T * nr; i += 32 * NW) {
+      const int m = i / nr, r = i - m * nr, n = n0 + r;
+      float v = 0.f;
 #pragma unroll
-      for (int w = 1; w < kStreamWarps; ++w) {
-        const float4 q = red[w][rt][mg][lane];
-        v.x += q.x;
-        v.y += q.y;
-        v.z += q.z;
-        v.w += q.w;
-      }
-      const float o[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + rt * 16 + g + (j >= 2 ? 8 : 0);
-        const int m = mg * 8 + 2 * t + (j & 1);
-        if (n >= n1 || m >= a.T) continue;
-        float r = o[j];
-        if (a.res) r += __half2float(a.res[m * a.ldr + n]);
-        a.y[m * a.ldy + n] = __float2half_rn(r);
-      }
+      for (int w = 0; w < NW; ++w) v += y_all[(w * a.T + m) * C::YROW + r];
+      if (a.res) v += __half2float(a.res[m * a.ldr + n]);
+      a.y[m * a.ldy + n] = __float2half_rn(v);
     }
     __syncthreads();
   }
@@ -671,42 +780,57 @@ namespace {
 
 size_t moe_plan_bytes() { return (sizeof(MoePlan) + 255) / 256 * 256; }
 
-cudaError_t launch_route(const __half* x, long long ldx, const __half* wr, long long ldw,
-                         const __half* bias, int T, int E, int H, int k, int normalize, int* ids,
-                         float* weights, MoePlan* plan, cudaStream_t st) {
-  const int tok = T <= 8 ? 8 : 32;
-  const dim3 grid((unsigned)((T + tok - 1) / tok * kRouteCluster));
-  auto kern = T <= 8 ? k_moe_route<1> : k_moe_route<4>;
-  return launch_ex(kern, grid, dim3(kStreamThreads), 0, st, kRouteCluster, x, ldx, wr, ldw, bias,
-                   T, E, H, k, normalize, ids, weights, plan);
+template <int MG>
+cudaError_t launch_route_mg(const RouteArgs& a, cudaStream_t st) {
+  using C = RouteCfg<MG>;
+  static BigSmem big;
+  const int grid = (a.T + C::TOK - 1) / C::TOK * kRouteCluster;
+  return launch_big(k_moe_route<MG>, big, C::SMEM, grid, 32 * C::NW, C::SMEM, st, kRouteCluster, a);
 }
 
+cudaError_t launch_route(const RouteArgs& a, cudaStream_t st) {
+  return a.T <= 8 ? launch_route_mg<1>(a, st) : launch_route_mg<4>(a, st);
+}
+
+template <int WQ, int MG, int RT>
+cudaError_t launch_down(const MoeArgs& a, int rows, int grid, cudaStream_t st) {
+  using C = DownCfg<WQ, MG, RT>;
+  static BigSmem big;
+  return launch_big(k_moe_down<WQ, MG, RT>, big, C::smem(C::MAX_T, C::MAX_T * kMoeMaxK),
+                    grid, 32 * C::NW, C::smem(a.T, rows), st, 1, a, rows);
+}
+
+// MG: groups of 8 columns a slot can have (1 up to 8 tokens, else 2).
 template <int WQ, int MG>
-cudaError_t launch_experts(const MoeArgs& a, cudaStream_t st) {
+cudaError_t launch_experts(const MoeArgs& a, int rows, cudaStream_t st) {
   const int sms = std::max(1, current_sms());
-  const int grid = 2 * sms;
-  cudaError_t e = launch_ex(k_moe_gate_up<WQ, MG, MG == 1 ? 4 : 2>, dim3(grid),
-                            dim3(kStreamThreads), 0, st, 1, a);
-  if (e != cudaSuccess) return e;
-  const int gd = std::min(grid, (a.H + 7) / 8);
-  const int rows = (a.H + gd - 1) / gd;
-  if (rows <= 16)
-    return launch_ex(k_moe_down<WQ, MG, 1>, dim3(gd), dim3(kStreamThreads), 0, st, 1, a);
-  return launch_ex(k_moe_down<WQ, MG, 2>, dim3(gd), dim3(kStreamThreads), 0, st, 1, a);
+  {
+    constexpr int RT = GU_RT;
+    using C = GateUpCfg<WQ, MG, RT>;
+    static BigSmem big;
+    const cudaError_t e =
+        launch_big(k_moe_gate_up<WQ, MG, RT>, big, C::SMEM + kMoeMaxRows * 12, sms,
+                   32 * C::NW, C::SMEM + rows * 12, st, 1, a, rows);
+    if (e != cudaSuccess) return e;
+  }
+  const int grid = std::min(sms, (a.H + 7) / 8);
+  const int per = (a.H + grid - 1) / grid;
+  if (per <= 16) return launch_down<WQ, MG, 1>(a, rows, grid, st);
+  if (per <= 32) return launch_down<WQ, MG, 2>(a, rows, grid, st);
+  return launch_down<WQ, MG, 3>(a, rows, grid, st);
 }
 
 template <int WQ>
-cudaError_t launch_experts_t(const MoeArgs& a, cudaStream_t st) {
-  if (a.T <= 8) return launch_experts<WQ, 1>(a, st);
-  if (a.T <= 16) return launch_experts<WQ, 2>(a, st);
-  return launch_experts<WQ, 4>(a, st);
+cudaError_t launch_experts_t(const MoeArgs& a, int rows, cudaStream_t st) {
+  return a.T <= 8 ? launch_experts<WQ, 1>(a, rows, st) : launch_experts<WQ, 2>(a, rows, st);
 }
 
-cudaError_t run_experts(const MoeArgs& a, int kind, cudaStream_t st) {
+cudaError_t run_experts(const MoeArgs& a, int top_k, int kind, cudaStream_t st) {
+  const int rows = a.T * top_k;
   switch (kind) {
-    case kWFp16: return launch_experts_t<0>(a, st);
-    case kWInt8PerChannel: return launch_experts_t<1>(a, st);
-    case kWUint8Group: return launch_experts_t<2>(a, st);
+    case kWFp16: return launch_experts_t<0>(a, rows, st);
+    case kWInt8PerChannel: return launch_experts_t<1>(a, rows, st);
+    case kWUint8Group: return launch_experts_t<2>(a, rows, st);
     default: return cudaErrorInvalidConfiguration;
   }
 }

@@ -22,7 +22,6 @@
 #include "elementwise.cuh"
 #include "collective.cuh"
 #include "epilogue.cuh"
-#include "moe.cuh"
 
 namespace tempo_sm100 {
 namespace {
@@ -59,57 +58,6 @@ int fill_epilogue(Problem& pr, const void* bias, const void* residual, int ldr, 
   if (bias && !aligned16(bias)) return cudaErrorInvalidConfiguration;
   if (residual && (!aligned16(residual) || ldr < pr.N || ldr % 8))
     return cudaErrorInvalidConfiguration;
-  return 0;
-}
-
-int route_args(const void* x, const void* wr, const int* ids, const float* weights, int T, int E,
-               int H, int k, int ldx, int ldw) {
-  if (!x || !wr || !ids || !weights || T < 1 || E < 1 || H < 1 || k < 1 || k > E)
-    return cudaErrorInvalidValue;
-  if (E > kMoeMaxE || k > kMoeMaxK || H % 8 || ldx < H || ldw < H || ldx % 8 || ldw % 8 ||
-      !aligned16(x) || !aligned16(wr))
-    return cudaErrorInvalidConfiguration;
-  return 0;
-}
-
-int moe_args(MoeArgs& a, const void* x, const void* wgu, const void* wd, const void* sgu,
-             const void* zgu, const void* sd, const void* zd, const void* res, void* y, int T,
-             int E, int H, int I, int k, int ldx, int ldr, int ldy, int kind, int group,
-             int gu_block, void* ws, size_t ws_bytes) {
-  if (!x || !wgu || !wd || !y || T < 1 || E < 1 || H < 1 || I < 1 || k < 1)
-    return cudaErrorInvalidValue;
-  if (kind < kWFp16 || kind > kWUint8Group || (kind && (!sgu || !sd)) ||
-      (kind == kWUint8Group && (!zgu || !zd)))
-    return cudaErrorInvalidValue;
-  if (T > kMoeMaxT || E > kMoeMaxE || k > kMoeMaxK || H % 16 || I % 16 || ldx < H || ldx % 8 ||
-      ldy < H || (res && ldr < H) || !aligned16(x) || !aligned16(wgu) || !aligned16(wd))
-    return cudaErrorInvalidConfiguration;
-  if (kind == kWUint8Group && (group <= 0 || group % 64 || H % group || I % group))
-    return cudaErrorInvalidConfiguration;
-  if (gu_block < 0 || (gu_block && (gu_block % 8 || I % gu_block)))
-    return cudaErrorInvalidConfiguration;
-  if (!ws || !aligned16(ws) || ws_bytes < tempo_sm100_moe_workspace_bytes(T, k, I))
-    return cudaErrorInvalidValue;
-  a.x = static_cast<const __half*>(x);
-  a.ldx = ldx;
-  a.T = T;
-  a.E = E;
-  a.H = H;
-  a.I = I;
-  a.wgu = static_cast<const uint8_t*>(wgu);
-  a.wd = static_cast<const uint8_t*>(wd);
-  a.sgu = static_cast<const __half*>(sgu);
-  a.sd = static_cast<const __half*>(sd);
-  a.zgu = static_cast<const uint8_t*>(zgu);
-  a.zd = static_cast<const uint8_t*>(zd);
-  a.group = group > 0 ? group : 1;
-  a.gu_block = gu_block;
-  a.plan = static_cast<MoePlan*>(ws);
-  a.h = reinterpret_cast<float*>(static_cast<char*>(ws) + moe_plan_bytes());
-  a.res = static_cast<const __half*>(res);
-  a.ldr = ldr;
-  a.y = static_cast<__half*>(y);
-  a.ldy = ldy;
   return 0;
 }
 
@@ -321,60 +269,6 @@ int tempo_sm100_gemm_w8a16_epilogue(const void* A, const void* W, const void* sc
              ws ? ws_bytes : 0};
   const int rc = fill_epilogue(pr, bias, residual, ldr, activation);
   return rc ? rc : run_epilogue(pr, static_cast<cudaStream_t>(stream));
-}
-
-int tempo_sm100_moe_route(const void* x, const void* w_router, const void* bias, int* ids,
-                          float* weights, int T, int E, int H, int top_k, int ldx, int ldw,
-                          int normalize, void* stream) {
-  const int rc = route_args(x, w_router, ids, weights, T, E, H, top_k, ldx, ldw);
-  if (rc) return rc;
-  return launch_route(static_cast<const __half*>(x), ldx, static_cast<const __half*>(w_router),
-                      ldw, static_cast<const __half*>(bias), T, E, H, top_k, normalize, ids,
-                      weights, nullptr, static_cast<cudaStream_t>(stream));
-}
-
-size_t tempo_sm100_moe_workspace_bytes(int T, int top_k, int I) {
-  if (T < 1 || top_k < 1 || I < 1) return 0;
-  return moe_plan_bytes() + (size_t)T * top_k * I * sizeof(float);
-}
-
-int tempo_sm100_moe_layer(const void* x, const void* w_router, const void* bias,
-                          const void* w_gate_up, const void* w_down, const void* s_gate_up,
-                          const void* z_gate_up, const void* s_down, const void* z_down,
-                          const void* residual, void* y, int* ids, float* weights, int T, int E,
-                          int H, int I, int top_k, int ldx, int ldw, int ldr, int ldy,
-                          int weight_kind, int group_size, int gu_block, int normalize, void* ws,
-                          size_t ws_bytes, void* stream) {
-  int rc = route_args(x, w_router, ids, weights, T, E, H, top_k, ldx, ldw);
-  if (rc) return rc;
-  MoeArgs a{};
-  rc = moe_args(a, x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, residual, y, T, E,
-                H, I, top_k, ldx, ldr, ldy, weight_kind, group_size, gu_block, ws, ws_bytes);
-  if (rc) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e =
-      launch_route(a.x, ldx, static_cast<const __half*>(w_router), ldw,
-                   static_cast<const __half*>(bias), T, E, H, top_k, normalize, ids, weights,
-                   a.plan, st);
-  return e != cudaSuccess ? e : run_experts(a, weight_kind, st);
-}
-
-int tempo_sm100_moe_experts(const void* x, const int* ids, const float* weights,
-                            const void* w_gate_up, const void* w_down, const void* s_gate_up,
-                            const void* z_gate_up, const void* s_down, const void* z_down,
-                            const void* residual, void* y, int T, int E, int H, int I, int top_k,
-                            int ldx, int ldr, int ldy, int weight_kind, int group_size,
-                            int gu_block, void* ws, size_t ws_bytes, void* stream) {
-  if (!ids || !weights) return cudaErrorInvalidValue;
-  MoeArgs a{};
-  const int rc =
-      moe_args(a, x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, residual, y, T, E,
-               H, I, top_k, ldx, ldr, ldy, weight_kind, group_size, gu_block, ws, ws_bytes);
-  if (rc) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = launch_ex(k_moe_plan, dim3(1), dim3(kStreamThreads), 0, st, 1, ids,
-                                  weights, T, top_k, E, a.plan);
-  return e != cudaSuccess ? e : run_experts(a, weight_kind, st);
 }
 
 int tempo_sm100_ipc_alloc(size_t bytes, void** out_ptr) {

@@ -67,7 +67,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 
 // Bounded wait.  Returns false if the CTA-wide abort flag is raised or the time limit passes;
 // on a timeout the first failing block records itself in g_status and raises the abort flag.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                             int where) {
   const uint64_t t0 = globaltimer();
   while (true) {
@@ -306,7 +306,7 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
 }
 
 // Bounded wait with cluster-scope acquire (arrivals may come from the peer CTA).
-__device__ __noinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
+static __device__ __noinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
                                                volatile int* abort_flag, int where) {
   if (mbar_try_wait_cluster(bar, parity)) return true;
   const uint64_t t0 = globaltimer();
@@ -342,7 +342,7 @@ __device__ __forceinline__ bool mbar_test_wait_cluster(uint32_t bar, uint32_t pa
 }
 
 // Bounded polling wait (test_wait) with cluster-scope acquire.
-__device__ __noinline__ bool mbar_poll_cluster(uint32_t bar, uint32_t parity,
+static __device__ __noinline__ bool mbar_poll_cluster(uint32_t bar, uint32_t parity,
                                                volatile int* abort_flag, int where) {
   const uint64_t t0 = globaltimer();
   while (true) {
