@@ -37,9 +37,9 @@ constexpr int kPlanThreads = 256;
 struct MoePlan {
   int n_slots;                      // every slot has a token, so at most T * top_k
   int pad[3];
-  int expert[kMoeMaxRows];          // slot -> expert, ascending
-  int base[kMoeMaxRows];            // slot -> its first row; column c is row base + c
-  unsigned mask[kMoeMaxRows];       // slot -> its tokens; column c is the c-th set bit
+  int meta[kMoeMaxRows];            // slot -> expert (ascending) | number of its rows << 16
+  int base[kMoeMaxRows];            // slot -> its first row
+  unsigned char token[kMoeMaxRows]; // row -> token, ascending within an expert
   float weight[kMoeMaxRows];        // row -> routing weight
   unsigned amax[kMoeMaxRows];       // row -> bits of max |h| (k_moe_gate_up)
 };
@@ -92,9 +92,8 @@ __device__ void moe_build_plan(MoePlan* plan, const int* ids, const float* w, in
       for (unsigned left = m; left; ++s, b += kMoeCols) {
         unsigned rest = left;
         for (int i = 0; i < kMoeCols && rest; ++i) rest &= rest - 1u;
-        plan->expert[s] = e;
+        plan->meta[s] = e | __popc(left & ~rest) << 16;
         plan->base[s] = b;
-        plan->mask[s] = left & ~rest;
         left = rest;
       }
       const int all = __shfl_sync(0xffffffffu, incl, 31);
@@ -115,7 +114,10 @@ __device__ void moe_build_plan(MoePlan* plan, const int* ids, const float* w, in
       if (j < i) first = false;
       sum += w[j];
     }
-    if (first) plan->weight[ebase[e] + __popc(emask[e] & ((1u << t) - 1u))] = sum;
+    if (!first) continue;
+    const int row = ebase[e] + __popc(emask[e] & ((1u << t) - 1u));
+    plan->weight[row] = sum;
+    plan->token[row] = (unsigned char)t;
   }
 }
 
@@ -233,12 +235,6 @@ struct RouteJob {
                    a.x + (long long)(t0 + m) * a.ldx + kw + 8 * (lane & 3), ok);
     }
   }
-  __device__ __forceinline__ unsigned use_cols(const Piece&) const {
-    unsigned c = 0;
-#pragma unroll
-    for (int mg = 0; mg < MG; ++mg) c |= (mg * 8 + (lane >> 2) < nt ? 1u : 0u) << mg;
-    return c;
-  }
   __device__ __forceinline__ unsigned live(const Piece&) const {
     return (1u << ((nt + 7) / 8)) - 1u;
   }
@@ -264,7 +260,7 @@ struct RouteCfg {
   static constexpr int TOK = MG * 8;  // tokens of a cluster
   static constexpr int OWN = (TOK + kRouteCluster - 1) / kRouteCluster;
   using F = StreamFifo<kWFp16, MG, 1, 1>;
-  static constexpr int RED = 8 * MG * 512;
+  static constexpr int RED = NW * MG * 512;
   static constexpr int REST = OWN * kMoeMaxE * 4 + 2 * kMoeMaxRows * 4 + 2 * kMoeMaxE * 4;
   static constexpr int S = F::depth((kMaxDynSmem - RED - REST) / NW);
   static constexpr int FIFO = NW * S * F::STAGE;
@@ -296,7 +292,7 @@ __global__ void __launch_bounds__(32 * RouteCfg<MG>::NW, 1) k_moe_route(const Ro
                    logits};
   stream_run<kWFp16, MG, 1, 1, C::NW, C::S, true>(
       job, smem, reinterpret_cast<float4*>(smem + C::FIFO),
-      (a.H + StreamStep<kWFp16>::STEP - 1) / StreamStep<kWFp16>::STEP);
+      (a.H + StreamStep<kWFp16>::STEP - 1) / StreamStep<kWFp16>::STEP, stream_worker<C::NW>(C::NW));
   cluster_sync();
   for (int q = warp; q < C::OWN; q += C::NW) {
     const int m = q * kRouteCluster + rank;
@@ -337,28 +333,28 @@ __device__ __forceinline__ int gate_row(int c, int block) {
   return block ? (c / block) * 2 * block + c % block : c;
 }
 
-// The plan's slots in shared memory, for kernels that look them up as they go.
+// The plan's slots and rows in shared memory, for kernels that look them up as they go.
 struct SlotTable {
-  int* expert;
+  int* meta;
   int* base;
-  unsigned* mask;
+  unsigned char* token;
+  static constexpr int BYTES = 9;  // per row
   __device__ __forceinline__ SlotTable(uint8_t* smem, int rows)
-      : expert(reinterpret_cast<int*>(smem)), base(expert + rows),
-        mask(reinterpret_cast<unsigned*>(base + rows)) {}
-  __device__ __forceinline__ void load(const MoePlan& p, int n_slots) {
-    for (int i = threadIdx.x; i < n_slots; i += blockDim.x) {
-      expert[i] = p.expert[i];
+      : meta(reinterpret_cast<int*>(smem)), base(meta + rows),
+        token(reinterpret_cast<unsigned char*>(base + rows)) {}
+  // All rows' entries, whatever the number of slots: it is read at the same time.
+  __device__ __forceinline__ int load(const MoePlan& p, int rows) {
+    const int n_slots = p.n_slots;
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+      meta[i] = p.meta[i];
       base[i] = p.base[i];
-      mask[i] = p.mask[i];
+      token[i] = p.token[i];
     }
+    return n_slots;
   }
+  __device__ __forceinline__ int expert(int slot) const { return meta[slot] & 0xffff; }
+  __device__ __forceinline__ int cols(int slot) const { return meta[slot] >> 16; }
 };
-
-// Token of column c of a slot (the c-th set bit); -1 past its last.
-__device__ __forceinline__ int slot_token(unsigned mask, int c) {
-  for (int i = 0; i < c && mask; ++i) mask &= mask - 1u;
-  return __ffs((int)mask) - 1;
-}
 
 // A row tile is 8 columns of h: MMA rows 0-7 are their gate rows, rows 8-15 their up rows, so
 // silu(gate) * up needs no exchange.  CTA b of G owns the quads of columns [n b / G, n (b + 1) / G)
@@ -372,47 +368,82 @@ struct GateUpJob {
   static constexpr bool ROTATE = true;
   const MoeArgs& a;
   const SlotTable& tab;
-  long long lo, hi;
+  int lo, hi;  // quads of columns, all slots' in one sequence
   int lane, up, per_slot;
   long long up_bytes;  // from a gate row to its up row
   unsigned per_group;  // group_magic
   struct Piece {
-    long long end;        // first quad after the piece
-    int slot, c0, c1;     // its columns
-    unsigned mask;
-    int tok[MG];          // token of this lane's column of each group, or -1
+    int slot, q, left;    // first quad in the slot; quads of the worker from it on
+    int c0, c1;           // columns
+    int expert, base, n_cols;
     const uint8_t* w[RT];  // this lane's chunk of each tile's gate row at k = 0
     const __half* x[MG];   // vector lane % 4 of the token of column lane / 4
-    long long z;           // group-wise: where the slot's scales and zero points start
+    GroupWord z[WQ == kWUint8Group ? RT : 1];
   };
-  __device__ __forceinline__ bool at(Piece& p, long long pos) const {
-    if (pos >= hi) return false;
-    p.slot = (int)(pos / per_slot);
-    const int q = (int)(pos - (long long)p.slot * per_slot);
-    const int left = (int)min((long long)(per_slot - q), hi - pos);
+  __device__ __forceinline__ void enter_slot(Piece& p) const {
+    p.expert = tab.expert(p.slot);
+    p.base = tab.base[p.slot];
+    p.n_cols = tab.cols(p.slot);
+#pragma unroll
+    for (int mg = 0; mg < MG; ++mg) {
+      const int c = mg * 8 + (lane >> 2);
+      p.x[mg] = a.x + (c < p.n_cols ? tab.token[p.base + c] : 0) * a.ldx + 8 * (lane & 3);
+    }
+  }
+  __device__ __forceinline__ bool enter(Piece& p) const {
+    if (p.left <= 0) return false;
+    const int left = min(per_slot - p.q, p.left);
     const int np = (left + 2 * RT - 1) / (2 * RT);
     const int cnt = (left + np - 1) / np;
-    p.c0 = 4 * q;
-    p.c1 = 4 * (q + cnt);
-    p.end = pos + cnt;
-    p.mask = tab.mask[p.slot];
-    const long long e = tab.expert[p.slot];
+    p.c0 = 4 * p.q;
+    p.c1 = 4 * (p.q + cnt);
+    const long long e = p.expert;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       // past the piece's columns the last one's row (never copied)
       const int c = min(p.c0 + rt * 8 + (lane >> 2), p.c1 - 1);
       p.w[rt] = a.wgu + ((e * 2 * a.I + gate_row(c, a.gu_block)) * a.H + (lane & 3) * St::KC) * St::ESZ;
     }
+    if (WQ == kWUint8Group) {
+      // a tile's scales and zero points: 8 gate rows, then 8 up rows (columns come in quads and
+      // blocks of rows are multiples of 8, so every word is aligned): two scales each of lanes
+      // 0-7, four zero points each of lanes kZeroLane ..+ 3
+      const bool sc = lane < kZeroLane;
+      const int half = sc ? lane >> 2 : (lane - kZeroLane) >> 1;
+      const int at = sc ? 2 * (lane & 3) : 4 * ((lane - kZeroLane) & 1);
+      const long long z0 = e * (a.H / a.group) * 2 * a.I;
 #pragma unroll
-    for (int mg = 0; mg < MG; ++mg) {
-      p.tok[mg] = slot_token(p.mask, mg * 8 + (lane >> 2));
-      p.x[mg] = a.x + max(p.tok[mg], 0) * a.ldx + 8 * (lane & 3);
+      for (int rt = 0; rt < RT; ++rt) {
+        const int c = p.c0 + rt * 8 + at;
+        const bool on = half < 2 && c < p.c1;
+        const long long r = z0 + (on ? gate_row(c, a.gu_block) + half * up : 0);
+        p.z[WQ == kWUint8Group ? rt : 0] = {
+            sc ? reinterpret_cast<const uint8_t*>(a.sgu + r) : a.zgu + r,
+            on ? (sc ? 4u : 2u) * a.I : 0u};
+      }
     }
-    if (WQ == kWUint8Group) p.z = e * (a.H / a.group) * 2 * a.I;
     return true;
   }
-  __device__ __forceinline__ bool first(Piece& p) const { return at(p, lo); }
-  __device__ __forceinline__ bool next(Piece& p) const { return at(p, p.end); }
+  __device__ __forceinline__ bool first(Piece& p) const {
+    p.left = hi - lo;
+    if (p.left <= 0) return false;
+    p.slot = lo / per_slot;
+    p.q = lo - p.slot * per_slot;
+    enter_slot(p);
+    return enter(p);
+  }
+  __device__ __forceinline__ bool next(Piece& p) const {
+    const int cnt = (p.c1 - p.c0) >> 2;
+    p.left -= cnt;
+    if (p.left <= 0) return false;
+    p.q += cnt;
+    if (p.q == per_slot) {
+      p.q = 0;
+      ++p.slot;
+      enter_slot(p);
+    }
+    return enter(p);
+  }
   __device__ __forceinline__ void copy(const Piece& p, int step, uint32_t stage) const {
     const int kw = step * St::STEP;
     const bool ok = kw + (lane & 3) * St::KC < a.H;
@@ -426,26 +457,13 @@ struct GateUpJob {
         cp_async16(d, src, ok);
         cp_async16(d + 512, src + up_bytes, ok);
       }
-      if (WQ == kWUint8Group) {
-        // 8 gate and 8 up rows: lanes 0-7 two scales each, lanes 16-19 four zero points (columns
-        // come in quads, blocks of rows are multiples of 8)
-        const long long gi = p.z + (long long)step_group(step, per_group) * 2 * a.I;
-        const uint32_t z = stage + F::Z_OFF + rt * 128;
-        if (lane < 8) {
-          const int cc = c + 2 * (lane & 3);
-          if (cc < p.c1)
-            cp_async4(z + 4 * lane, a.sgu + gi + gate_row(cc, a.gu_block) + (lane < 4 ? 0 : up), true);
-        } else if (lane >= 16 && lane < 20) {
-          const int cc = c + 4 * (lane & 1);
-          if (cc < p.c1)
-            cp_async4(z + 64 + 4 * (lane - 16),
-                      a.zgu + gi + gate_row(cc, a.gu_block) + (lane < 18 ? 0 : up), true);
-        }
-      }
+      if (WQ == kWUint8Group)
+        copy_group_word(stage + F::Z_OFF + rt * 128, p.z[WQ == kWUint8Group ? rt : 0],
+                        step_group(step, per_group), lane);
     }
 #pragma unroll
     for (int mg = 0; mg < MG; ++mg) {
-      if (p.tok[mg] >= 0) {
+      if (mg * 8 + (lane >> 2) < p.n_cols) {
 #pragma unroll
         for (int v = 0; v < St::NB / 4; ++v)
           cp_async16(stage + F::B_OFF + b_vec<St::NB / 4>(mg, 4 * v + (lane & 3), lane >> 2),
@@ -453,28 +471,22 @@ struct GateUpJob {
       }
     }
   }
-  __device__ __forceinline__ unsigned use_cols(const Piece& p) const {
-    unsigned c = 0;
-#pragma unroll
-    for (int mg = 0; mg < MG; ++mg) c |= (p.tok[mg] >= 0 ? 1u : 0u) << mg;
-    return c;
-  }
   __device__ __forceinline__ unsigned live(const Piece& p) const {
-    return __popc(p.mask) > 8 ? 3u : 1u;
+    return p.n_cols > 8 ? 3u : 1u;
   }
   __device__ __forceinline__ void z_rows(const Piece&, int (&r)[RT]) const {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) r[rt] = 0;
   }
   __device__ __forceinline__ void finish(const Piece& p, int rt, int mg, float4 v) const {
-    const int n_cols = __popc(p.mask);
+    const int n_cols = p.n_cols;
     if (p.c0 + rt * 8 >= p.c1 || mg * 8 >= n_cols) return;  // warp-uniform
     const int g = lane >> 2, t = lane & 3;
     const int c = p.c0 + rt * 8 + g;
     const bool in = c < p.c1;
     float sg = 1.f, su = 1.f;
     if (WQ == kWInt8PerChannel && in) {
-      const __half* sc = a.sgu + (long long)tab.expert[p.slot] * 2 * a.I + gate_row(c, a.gu_block);
+      const __half* sc = a.sgu + (long long)p.expert * 2 * a.I + gate_row(c, a.gu_block);
       sg = __half2float(__ldg(sc));
       su = __half2float(__ldg(sc + up));
     }
@@ -483,7 +495,7 @@ struct GateUpJob {
     for (int j = 0; j < 2; ++j) {
       const int col = mg * 8 + 2 * t + j;
       const bool on = col < n_cols;
-      const int row = tab.base[p.slot] + col;
+      const int row = p.base + col;
       float hv = 0.f;
       if (on && in) {
         hv = gt[j] / (1.f + expf(-gt[j])) * ut[j] * a.plan->weight[row];
@@ -500,37 +512,39 @@ struct GateUpJob {
 
 template <int WQ, int MG, int RT>
 struct GateUpCfg {
-  static constexpr int NW = GU_NW;
+  static constexpr int NW = 16;
   static constexpr int BV = StreamStep<WQ>::NB / 4;
   using F = StreamFifo<WQ, MG, RT, BV>;
-  static constexpr int RED = 8 * RT * MG * 512;
-  static constexpr int S = F::depth((kMaxDynSmem - RED - kMoeMaxRows * 12) / NW);
+  static constexpr int RED = NW * RT * MG * 512;
+  static constexpr int TABLE = kMoeMaxRows * SlotTable::BYTES;
+  static constexpr int S = F::depth((kMaxDynSmem - RED - TABLE) / NW);
   static constexpr int FIFO = NW * S * F::STAGE;
   static constexpr int SMEM = FIFO + RED;  // + the slot table
-  static_assert(SMEM + kMoeMaxRows * 12 <= kMaxDynSmem, "shared memory");
+  static_assert(SMEM + TABLE <= kMaxDynSmem, "shared memory");
 };
 
 template <int WQ, int MG, int RT>
 __global__ void __launch_bounds__(32 * GateUpCfg<WQ, MG, RT>::NW, 1)
-    k_moe_gate_up(const MoeArgs a, int rows) {
+    k_moe_gate_up(const MoeArgs a, int rows, int ks) {
   using C = GateUpCfg<WQ, MG, RT>;
   extern __shared__ __align__(16) uint8_t smem[];
   SlotTable tab(smem + C::SMEM, rows);
   pdl_wait();
   pdl_launch_dependents();
-  const int n_slots = a.plan->n_slots;
-  tab.load(*a.plan, n_slots);
+  const int n_slots = tab.load(*a.plan, rows);
   __syncthreads();
+  const StreamWorker wk = stream_worker<C::NW>(ks);
   const int per_slot = a.I / 4;
-  const long long n = (long long)n_slots * per_slot;
-  GateUpJob<WQ, MG, RT> job{a, tab, n * blockIdx.x / gridDim.x, n * (blockIdx.x + 1) / gridDim.x,
+  int lo, hi;
+  split_even(n_slots * per_slot, wk.id, wk.count, lo, hi);
+  GateUpJob<WQ, MG, RT> job{a, tab, lo, hi,
                             (int)(threadIdx.x & 31), a.gu_block ? a.gu_block : a.I, per_slot,
                             (long long)(a.gu_block ? a.gu_block : a.I) * a.H *
                                 StreamStep<WQ>::ESZ,
                             group_magic<WQ>(a.group)};
   stream_run<WQ, MG, RT, C::BV, C::NW, C::S>(
       job, smem, reinterpret_cast<float4*>(smem + C::FIFO),
-      (a.H + StreamStep<WQ>::STEP - 1) / StreamStep<WQ>::STEP);
+      (a.H + StreamStep<WQ>::STEP - 1) / StreamStep<WQ>::STEP, wk);
 }
 
 // s such that 2^s takes a largest value with these bits to [2^14, 2^15); 0 for zero.
@@ -551,17 +565,17 @@ __device__ __forceinline__ float pow2f(int s) { return __int_as_float((127 + s) 
 template <int WQ, int MG, int RT>
 struct DownCfg {
   using St = StreamStep<WQ>;
-  static constexpr int NW = MG == 1 ? DN_NW : DN_NW2;  // the sums of 32 tokens leave room for 8 warps
+  static constexpr int NW = MG == 1 ? 16 : 8;  // the sums of 32 tokens leave room for 8 warps
   static constexpr int MAX_T = MG == 1 ? 8 : kMoeMaxT;
   static constexpr int HV = St::KC / 4;  // 16-byte vectors of an fp32 chunk
   using F = StreamFifo<WQ, 1, RT, HV>;
   static constexpr int YROW = RT * 16 + 8;  // floats per token (padded: 4 tokens, 4 bank groups)
   __host__ __device__ static constexpr int y_bytes(int T) { return NW * T * YROW * 4; }
-  static constexpr int TABLE = MAX_T * kMoeMaxK * 13 + 16;
+  static constexpr int TABLE = MAX_T * kMoeMaxK * 10 + 16;
   static constexpr int S = F::depth((kMaxDynSmem - y_bytes(MAX_T) - TABLE) / NW);
   static constexpr int FIFO = NW * S * F::STAGE;
   __host__ __device__ static constexpr int smem(int T, int rows) {
-    return FIFO + y_bytes(T) + rows * 13 + 16;
+    return FIFO + y_bytes(T) + rows * 10 + 16;
   }
   static_assert(FIFO + y_bytes(MAX_T) + TABLE <= kMaxDynSmem, "shared memory");
 };
@@ -576,29 +590,35 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
   extern __shared__ __align__(16) uint8_t smem[];
   float* y_all = reinterpret_cast<float*>(smem + C::FIFO);
   SlotTable tab(smem + C::FIFO + C::y_bytes(a.T), rows);
-  signed char* shift = reinterpret_cast<signed char*>(tab.mask + rows);
+  signed char* shift = reinterpret_cast<signed char*>(tab.token + rows);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   // The plan may be read before the wait: k_moe_gate_up lets this grid start only after its own
   // wait, when the router (and all before it) had finished.  So the first steps' weights are
   // fetched here, under the rest of k_moe_gate_up; only h and its largest values need the wait.
-  const int n_slots = a.plan->n_slots;
-  tab.load(*a.plan, n_slots);
+  const int n_slots = tab.load(*a.plan, rows);
   __syncthreads();
-  const int lo = (int)((long long)a.H * blockIdx.x / gridDim.x);
-  const int hi = (int)((long long)a.H * (blockIdx.x + 1) / gridDim.x);
+  int lo, hi;
+  split_even(a.H, blockIdx.x, gridDim.x, lo, hi);
   const int nsteps = (a.I + St::STEP - 1) / St::STEP;
   const int npieces = (hi - lo + 16 * RT - 1) / (16 * RT);
   float* y = y_all + warp * a.T * C::YROW;
-  const uint32_t fifo = smem_u32(smem) + warp * S * F::STAGE;
-  // the warp's next step in the sequence of all slots' steps
-  const int rot = (int)((long long)nsteps * blockIdx.x / gridDim.x);
-  auto advance = [&](int& slot, int& step) {
-    step += NW;
-    while (step >= nsteps) {
-      step -= nsteps;
-      ++slot;
-    }
+  const uint8_t* fifo_p = smem + warp * S * F::STAGE;
+  const uint32_t fifo = smem_u32(fifo_p);
+  const int rot = (int)((unsigned)(nsteps * blockIdx.x) / gridDim.x);
+  // The warp's share of the sequence of all slots' steps: one run of them, so that it meets few
+  // slots and adds few sums to its tokens' (steps dealt out in turn instead: one token through 8
+  // int8 experts 77 us, so 71).
+  const int run = (n_slots * nsteps + NW - 1) / NW;
+  struct At {
+    int slot, step, left;  // left: steps of the run from here on
+  };
+  auto advance = [&](At& p) {  // -> whether the slot changed
+    --p.left;
+    if (++p.step < nsteps) return false;
+    p.step = 0;
+    ++p.slot;
+    return true;
   };
   auto k_of = [&](int step) {  // this lane's first k of a step (rotated as in stream_run)
     const int s = step + rot;
@@ -612,55 +632,72 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
     const long long row_bytes = (long long)a.I * St::ESZ;
     const uint8_t* w0 = a.wd + (n0 + g) * row_bytes + t * 16;
     const unsigned magic = group_magic<WQ>(a.group);
-    int lslot = 0, lstep = warp, lfifo = 0;
-    while (lstep >= nsteps) {
-      lstep -= nsteps;
-      ++lslot;
-    }
-    int uslot = lslot, ustep = lstep;
+    const int first = warp * run;
+    At l{first / nsteps, first % nsteps, min(run, n_slots * nsteps - first)};
+    At u = l;
+    int lfifo = 0;
+    // the slot being copied: this lane's chunks at k = 0
+    const uint8_t* lw;
+    const float* lh;
+    GroupWord lz[WQ == kWUint8Group ? RT : 1];
+    bool lon;
+    auto enter = [&]() {
+      if (l.left <= 0) return;
+      const long long e = tab.expert(l.slot);
+      lw = w0 + e * a.H * row_bytes;
+      lh = a.h + (long long)(tab.base[l.slot] + g) * a.I + 4 * t;
+      lon = g < tab.cols(l.slot);
+      if (WQ == kWUint8Group) {
+        const long long z0 = e * (a.I / a.group) * a.H;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          lz[WQ == kWUint8Group ? rt : 0] =
+              group_word(a.sd + z0, a.zd + z0, n0 + rt * 16, a.H, lane);
+      }
+    };
+    enter();
+    const long long row8 = 8 * row_bytes;
     auto issue = [&](bool weights, bool hidden) {
-      if (lslot < n_slots) {
-        const int step = lstep + rot < nsteps ? lstep + rot : lstep + rot - nsteps;
+      if (l.left > 0) {
+        const int step = l.step + rot < nsteps ? l.step + rot : l.step + rot - nsteps;
         const int kw = step * St::STEP;
-        const int e = tab.expert[lslot];
         const uint32_t stage = fifo + lfifo * F::STAGE;
         if (weights) {
           const bool ok = kw + t * St::KC < a.I;
-          const uint8_t* src = w0 + ((long long)e * a.H * row_bytes + kw * St::ESZ);
+          const uint8_t* src = lw + kw * St::ESZ;
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
             const int ra = n0 + rt * 16 + g;
             const uint32_t d = stage + rt * 1024 + lane * 16;
             // rows past the piece are never stored
-            if (ra < n1) cp_async16(d, src + 2 * rt * 8 * row_bytes, ok);
-            if (ra + 8 < n1) cp_async16(d + 512, src + (2 * rt + 1) * 8 * row_bytes, ok);
-            if (WQ == kWUint8Group) {
-              const long long gi =
-                  ((long long)e * (a.I / a.group) + step_group(step, magic)) * a.H;
-              copy_group_row(stage + F::Z_OFF + rt * 128, a.sd + gi, a.zd + gi, n0 + rt * 16,
-                             a.H, lane, true);
-            }
+            if (ra < n1) cp_async16(d, src, ok);
+            src += row8;
+            if (ra + 8 < n1) cp_async16(d + 512, src, ok);
+            src += row8;
+            if (WQ == kWUint8Group)
+              copy_group_word(stage + F::Z_OFF + rt * 128, lz[WQ == kWUint8Group ? rt : 0],
+                              step_group(step, magic), lane);
           }
         }
-        if (hidden && g < __popc(tab.mask[lslot])) {
-          const float* h = a.h + (long long)(tab.base[lslot] + g) * a.I + kw + 4 * t;
+        if (hidden && lon) {
+          const float* h = lh + kw;
 #pragma unroll
           for (int v = 0; v < HV; ++v)
             cp_async16(stage + F::B_OFF + b_vec<HV>(0, 4 * v + t, g), h + 16 * v,
                        kw + 16 * v + 4 * t < a.I);
         }
-        advance(lslot, lstep);
+        if (advance(l)) enter();
       }
       if (hidden) cp_async_commit();
       lfifo = lfifo + 1 == S ? 0 : lfifo + 1;
     };
     if (pc == 0) {
-      const int lslot0 = lslot, lstep0 = lstep;
+      const At l0 = l;
 #pragma unroll 1
       for (int i = 0; i < S - 1; ++i) issue(true, false);
-      lslot = lslot0;
-      lstep = lstep0;
+      l = l0;
       lfifo = 0;
+      enter();
       pdl_wait();
       pdl_launch_dependents();
       for (int i = tid; i < rows; i += 32 * NW)
@@ -676,10 +713,9 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
     int z_row[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) z_row[rt] = n0 + rt * 16;
-    while (uslot < n_slots) {
-      const int slot = uslot;
-      const unsigned mask = tab.mask[slot];
-      const int base = tab.base[slot], n_cols = __popc(mask);
+    while (u.left > 0) {
+      const int slot = u.slot;
+      const int base = tab.base[slot], n_cols = tab.cols(slot);
       float up2[MG];  // 2^s of this lane's columns
       bool fin[MG];   // whether the row of h is finite: if not its low parts (inf - inf) are left out
 #pragma unroll
@@ -689,32 +725,28 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
         up2[mg] = fin[mg] ? pow2f(sh) : 1.f;
       }
       float acc[RT][MG][4] = {};
-      while (uslot == slot) {
+      while (u.left > 0 && u.slot == slot) {
         cp_async_wait<S - 2>();
         __syncwarp();
         issue(true, true);
-        const uint32_t stage = fifo + ufifo * F::STAGE;
+        const uint8_t* stage = fifo_p + ufifo * F::STAGE;
         StreamA<WQ, RT> w;
         stream_read_weights<WQ, RT>(w, stage, F::Z_OFF, z_row, lane);
 #pragma unroll
         for (int mg = 0; mg < MG; ++mg) {
           if (mg * 8 >= n_cols) continue;  // warp-uniform
-          uint32_t bh[St::NB], bl[St::NB];
-          const bool on = mg * 8 + g < n_cols;
+          uint32_t b[2][St::NB];  // high and low parts
 #pragma unroll
           for (int v = 0; v < HV; ++v) {
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (on) {
-              if (mg == 0) {
-                const uint4 q = lds16(stage + F::B_OFF + b_vec<HV>(0, HV * t + v, g));
-                x = make_float4(__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z),
-                                __uint_as_float(q.w));
-              } else {
-                const int k0 = k_of(ustep) + t * St::KC;
-                if (k0 < a.I)
-                  x = *reinterpret_cast<const float4*>(
-                      a.h + (long long)(base + mg * 8 + g) * a.I + k0 + 4 * v);
-              }
+            float4 x;  // a column without a row holds anything: it stays in its column
+            if (mg == 0) {
+              x = *reinterpret_cast<const float4*>(stage + F::B_OFF + b_vec<HV>(0, HV * t + v, g));
+            } else {
+              const int k0 = k_of(u.step) + t * St::KC;
+              x = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (mg * 8 + g < n_cols && k0 < a.I)
+                x = *reinterpret_cast<const float4*>(
+                    a.h + (long long)(base + mg * 8 + g) * a.I + k0 + 4 * v);
             }
             const float s4[4] = {x.x * up2[mg], x.y * up2[mg], x.z * up2[mg], x.w * up2[mg]};
 #pragma unroll
@@ -723,18 +755,18 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
               const float2 back = __half22float2(hi2);
               const __half2 lo2 =
                   __floats2half2_rn(s4[2 * i] - back.x, s4[2 * i + 1] - back.y);
-              bh[2 * v + i] = *reinterpret_cast<const uint32_t*>(&hi2);
-              bl[2 * v + i] = fin[mg] ? *reinterpret_cast<const uint32_t*>(&lo2) : 0u;
+              b[0][2 * v + i] = *reinterpret_cast<const uint32_t*>(&hi2);
+              b[1][2 * v + i] = fin[mg] ? *reinterpret_cast<const uint32_t*>(&lo2) : 0u;
             }
           }
+          float bias[4];
+          stream_bias<WQ>(b, bias);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            stream_mma<WQ, RT>(w, rt, bh, acc[rt][mg]);
-            stream_mma<WQ, RT>(w, rt, bl, acc[rt][mg]);
-          }
+          for (int rt = 0; rt < RT; ++rt)
+            stream_mma<WQ, RT, false>(w, rt, b, bias, acc[rt][mg]);
         }
         ufifo = ufifo + 1 == S ? 0 : ufifo + 1;
-        advance(uslot, ustep);
+        advance(u);
       }
       // the slot's sums: undo the row's power of two, apply the channel's scale
 #pragma unroll
@@ -743,7 +775,7 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
         for (int j = 0; j < 2; ++j) {
           const int col = mg * 8 + 2 * t + j;
           if (col >= n_cols) continue;
-          float* yt = y + slot_token(mask, col) * C::YROW;
+          float* yt = y + tab.token[base + col] * C::YROW;
           const int sh = shift[base + col];
           const float f = sh != kNotFinite ? pow2f(-sh) : 1.f;
 #pragma unroll
@@ -753,7 +785,7 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
               const int r = rt * 16 + 8 * half + g;
               float v = acc[rt][mg][2 * half + j] * f;
               if (WQ == kWInt8PerChannel && n0 + r < n1)
-                v *= __half2float(__ldg(a.sd + (long long)tab.expert[slot] * a.H + n0 + r));
+                v *= __half2float(__ldg(a.sd + (long long)tab.expert(slot) * a.H + n0 + r));
               yt[r] += v;
             }
           }
@@ -800,17 +832,24 @@ cudaError_t launch_down(const MoeArgs& a, int rows, int grid, cudaStream_t st) {
                     grid, 32 * C::NW, C::smem(a.T, rows), st, 1, a, rows);
 }
 
+// Warps of a k_moe_gate_up worker: with few steps to a row fewer warps share them (a piece's fixed
+// cost is then spread over more of each warp's steps).  Measured with 4 / 8 / 16: 7 tokens, uint8,
+// 32 steps: 42.7 / 43.2 / 47 us; one token, int8, 80 steps: 71.9 / 70.8 / 75; 32 tokens, fp16, 120
+// steps: 459 / 454 / 463.
+int gate_up_warps(int nsteps) { return nsteps >= 64 ? 8 : 4; }
+
 // MG: groups of 8 columns a slot can have (1 up to 8 tokens, else 2).
 template <int WQ, int MG>
 cudaError_t launch_experts(const MoeArgs& a, int rows, cudaStream_t st) {
   const int sms = std::max(1, current_sms());
   {
-    constexpr int RT = GU_RT;
+    constexpr int RT = 2;
     using C = GateUpCfg<WQ, MG, RT>;
     static BigSmem big;
     const cudaError_t e =
-        launch_big(k_moe_gate_up<WQ, MG, RT>, big, C::SMEM + kMoeMaxRows * 12, sms,
-                   32 * C::NW, C::SMEM + rows * 12, st, 1, a, rows);
+        launch_big(k_moe_gate_up<WQ, MG, RT>, big, C::SMEM + kMoeMaxRows * SlotTable::BYTES, sms,
+                   32 * C::NW, C::SMEM + rows * SlotTable::BYTES, st, 1, a, rows,
+                   gate_up_warps((a.H + StreamStep<WQ>::STEP - 1) / StreamStep<WQ>::STEP));
     if (e != cudaSuccess) return e;
   }
   const int grid = std::min(sms, (a.H + 7) / 8);

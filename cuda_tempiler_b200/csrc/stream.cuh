@@ -7,8 +7,8 @@
 // arithmetic has to cost nothing beside it: the products run on the warp tensor-core instruction
 // (m16n8k16, fp16 inputs, fp32 accumulators) with 16 weight rows as its M side and 8 activation
 // rows as its N side, operands straight from the registers the loads fill.  Sums are fp32
-// throughout; 8-bit weights enter as exact integers (q, or q - z) and their scale multiplies the
-// fp32 sum (per group of k, or per channel at the end), so no weight is rounded.
+// throughout; 8-bit weights enter as exact integers and their scale multiplies the fp32 sum (per
+// group of k, or per channel at the end), so no weight is rounded.
 //
 // Lane (g, t) = (lane / 4, lane % 4) holds the 16-byte chunk t of a step of 4 chunks of rows g
 // and g + 8.  Lanes with equal t hold equal k ranges, so taking a chunk's k values in storage
@@ -26,13 +26,6 @@
 #include <cstdint>
 
 #include "stream.h"
-#ifndef LIN_NW
-#define LIN_NW 16
-#define GU_NW 16
-#define GU_RT 2
-#define DN_NW 16
-#define DN_NW2 8
-#endif
 
 namespace tempo_sm100 {
 
@@ -45,11 +38,14 @@ struct StreamStep {
   static constexpr int NB = KC / 2;        // 32-bit registers of one activation chunk
 };
 
-// The exact fp16 values of a chunk in storage order: fp16 weights as they are, int8 q, or
-// uint8 q - z with zb = (1024 + z) in both halves.
+// The fp16 operands of a chunk in storage order: fp16 weights as they are; 8-bit weights as
+// 1024 + u, exact, with u the unsigned byte (int8 q: u = q + 128).  What that adds to a step's sum,
+// (1024 + 128 or z) x the sum of the step's activations, is taken off the sum instead of every
+// weight: the activations' sum is one more chain of MMAs for all row tiles together, the
+// subtraction from every weight half of the unpacking.  A step's sum is at most 64 products, so
+// what the cancellation costs (its terms are about 16 times the difference's) is some 2^-18 of it.
 template <int WQ>
-__device__ __forceinline__ void stream_unpack(uint4 x, __half2 zb,
-                                              uint32_t (&h)[StreamStep<WQ>::NB]) {
+__device__ __forceinline__ void stream_unpack(uint4 x, uint32_t (&h)[StreamStep<WQ>::NB]) {
   if constexpr (WQ == kWFp16) {
     h[0] = x.x;
     h[1] = x.y;
@@ -57,23 +53,29 @@ __device__ __forceinline__ void stream_unpack(uint4 x, __half2 zb,
     h[3] = x.w;
   } else {
     const uint32_t flip = WQ == kWInt8PerChannel ? 0x80808080u : 0u;
-    const __half2 bias =
-        WQ == kWInt8PerChannel ? __half2half2(__ushort_as_half(0x6480)) : zb;  // 1024 + 128, or z
-    __half2 v[8];
-    u8x4_to_h2x2_biased(x.x ^ flip, v[0], v[1]);
-    u8x4_to_h2x2_biased(x.y ^ flip, v[2], v[3]);
-    u8x4_to_h2x2_biased(x.z ^ flip, v[4], v[5]);
-    u8x4_to_h2x2_biased(x.w ^ flip, v[6], v[7]);
+    const uint32_t v[4] = {x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = __hsub2(v[i], bias);
-      h[i] = *reinterpret_cast<const uint32_t*>(&v[i]);
+    for (int i = 0; i < 4; ++i) {
+      h[2 * i] = __byte_perm(v[i], 0x64646464u, 0x5150);
+      h[2 * i + 1] = __byte_perm(v[i], 0x64646464u, 0x5352);
     }
   }
 }
 
-__device__ __forceinline__ __half2 zero_bias(uint8_t z) {
-  return __half2half2(__ushort_as_half((unsigned short)(0x6400u | z)));
+// d = a x b + c (not volatile: the compiler may move it)
+__device__ __forceinline__ void stream_mma_16816(float (&d)[4], uint32_t a0, uint32_t a1,
+                                                 uint32_t a2, uint32_t a3, uint32_t b0,
+                                                 uint32_t b1, float c0, float c1, float c2,
+                                                 float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void stream_mma_16816(float (&d)[4], uint32_t a0, uint32_t a1,
+                                                 uint32_t a2, uint32_t a3, uint32_t b0,
+                                                 uint32_t b1) {
+  stream_mma_16816(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -108,10 +110,8 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool o
                "r"(on ? 16 : 0)
                : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
-               "r"(on ? 4 : 0)
-               : "memory");
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -120,13 +120,8 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(a)
-               : "memory");
-  return v;
+__device__ __forceinline__ uint4 lds16(const uint8_t* p) {
+  return *reinterpret_cast<const uint4*>(p);
 }
 
 // Offset in a group's activations of vector c of column g.
@@ -136,119 +131,176 @@ __device__ __forceinline__ int b_vec(int mg, int c, int g) {
   return (mg * BV + (c >> 2)) * BLK + (g * 4 + (c & 3)) * 16;
 }
 
-// The 16 scales and zero points of rows [r0, r0 + 16) of one group row: lanes 0-8 copy the scales
-// two by two, lanes 16-20 the zero points four by four, from the aligned word below r0 on (rows of
-// the group arrays are multiples of 16 long, so an aligned word that starts inside one ends there).
-__device__ __forceinline__ void copy_group_row(uint32_t dst, const __half* scale,
-                                               const uint8_t* zero, int r0, int n_rows, int lane,
-                                               bool on) {
-  if (lane < 9) {
+// The scales and zero points of a row tile's 16 rows in one group row, one 4-byte word per lane:
+// scales two by two from lane 0, zero points four by four from lane kZeroLane, each from the aligned
+// word at or below the first row on.  A lane's word of group j is at src + j * step.
+constexpr int kZeroLane = 9;
+struct GroupWord {
+  const uint8_t* src;
+  unsigned step;  // bytes from one group row to the next; 0: this lane has no word
+};
+
+// Rows [r0, r0 + 16) of arrays [groups][n_rows] (n_rows a multiple of 16, so that an aligned word
+// that starts inside a group row ends there).
+__device__ __forceinline__ GroupWord group_word(const __half* scale, const uint8_t* zero, int r0,
+                                                int n_rows, int lane) {
+  if (lane < kZeroLane) {
     const int r = (r0 & ~1) + 2 * lane;
-    cp_async4(dst + 4 * lane, scale + (on && r < n_rows ? r : 0), on && r < n_rows);
-  } else if (lane >= 16 && lane < 21) {
-    const int r = (r0 & ~3) + 4 * (lane - 16);
-    cp_async4(dst + 64 + 4 * (lane - 16), zero + (on && r < n_rows ? r : 0), on && r < n_rows);
+    return {reinterpret_cast<const uint8_t*>(scale + r), r < n_rows ? 2u * n_rows : 0u};
   }
+  const int r = (r0 & ~3) + 4 * (lane - kZeroLane);
+  return {zero + r, lane < kZeroLane + 5 && r < n_rows ? (unsigned)n_rows : 0u};
+}
+__device__ __forceinline__ void copy_group_word(uint32_t dst, const GroupWord& w, int group,
+                                                int lane) {
+  if (w.step) cp_async4(dst + 4 * lane, w.src + (unsigned long long)w.step * (unsigned)group);
 }
 
-__device__ __forceinline__ void read_group_row(uint32_t src, int r0, int row, float& s, __half2& zb) {
-  unsigned short hs;
-  unsigned z;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(hs) : "r"(src + 2 * ((r0 & 1) + row)) : "memory");
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(src + 64 + (r0 & 3) + row) : "memory");
-  s = __half2float(__ushort_as_half(hs));
-  zb = zero_bias((uint8_t)z);
+// Scale and 1024 + zero point of `row` of the tile.
+__device__ __forceinline__ void read_group_row(const uint8_t* src, int r0, int row, float& s,
+                                               float& zb) {
+  s = __half2float(*reinterpret_cast<const __half*>(src + 2 * ((r0 & 1) + row)));
+  zb = __half2float(
+      __ushort_as_half((unsigned short)(0x6400u | src[4 * kZeroLane + (r0 & 3) + row])));
 }
 
 // A step's weights as MMA operands (and, group-wise, the scales of the lane's two rows).
 template <int WQ, int RT>
 struct StreamA {
   uint32_t a[RT][StreamStep<WQ>::NB], b[RT][StreamStep<WQ>::NB];
+  // group-wise: scale and 1024 + zero point of the two rows
   float fa[WQ == kWUint8Group ? RT : 1], fb[WQ == kWUint8Group ? RT : 1];
+  float za[WQ == kWUint8Group ? RT : 1], zb[WQ == kWUint8Group ? RT : 1];
 };
 
 template <int WQ, int RT>
-__device__ __forceinline__ void stream_read_weights(StreamA<WQ, RT>& o, uint32_t stage,
+__device__ __forceinline__ void stream_read_weights(StreamA<WQ, RT>& o, const uint8_t* stage,
                                                     uint32_t z_off, const int (&z_row)[RT],
                                                     int lane) {
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const uint4 xa = lds16(stage + rt * 1024 + lane * 16);
     const uint4 xb = lds16(stage + rt * 1024 + 512 + lane * 16);
-    __half2 za = __float2half2_rn(0.f), zb = za;
     if constexpr (WQ == kWUint8Group) {
-      read_group_row(stage + z_off + rt * 128, z_row[rt], lane >> 2, o.fa[rt], za);
-      read_group_row(stage + z_off + rt * 128, z_row[rt], (lane >> 2) + 8, o.fb[rt], zb);
+      read_group_row(stage + z_off + rt * 128, z_row[rt], lane >> 2, o.fa[rt], o.za[rt]);
+      read_group_row(stage + z_off + rt * 128, z_row[rt], (lane >> 2) + 8, o.fb[rt], o.zb[rt]);
     }
-    stream_unpack<WQ>(xa, za, o.a[rt]);
-    stream_unpack<WQ>(xb, zb, o.b[rt]);
+    stream_unpack<WQ>(xa, o.a[rt]);
+    stream_unpack<WQ>(xb, o.b[rt]);
   }
 }
 
-// acc += weights of row tile rt x one activation chunk; group-wise the step's sum is scaled first.
-// STEPS: the step's sum starts at zero and is added in fp32.  A tensor core truncates what it adds
-// to a large accumulator; over a long K that shows in fp32 results (not in fp16 ones).
-template <int WQ, int RT, bool STEPS = false>
-__device__ __forceinline__ void stream_mma(const StreamA<WQ, RT>& w, int rt,
-                                           const uint32_t (&b)[StreamStep<WQ>::NB],
-                                           float (&acc)[4]) {
-  using S = StreamStep<WQ>;
-  if constexpr (WQ == kWUint8Group || STEPS) {
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
+// What stream_mma subtracts for a step's activation chunks b (N of them: their values add up):
+// int8: -1152 x the sum of each column (d[0], d[1]: columns 2t, 2t + 1); uint8: the sum itself.
+template <int WQ, int N>
+__device__ __forceinline__ void stream_bias(const uint32_t (&b)[N][StreamStep<WQ>::NB],
+                                            float (&d)[4]) {
+  if constexpr (WQ != kWFp16) {
+    const uint32_t c = WQ == kWInt8PerChannel ? 0xE480E480u : 0x3C003C00u;  // -1152 or 1
+    stream_mma_16816(d, c, c, c, c, b[0][0], b[0][1], 0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < S::NMMA; ++j)
-      mma_16816(d, w.a[rt][2 * j], w.b[rt][2 * j], w.a[rt][2 * j + 1], w.b[rt][2 * j + 1],
-                b[2 * j], b[2 * j + 1]);
-    const float fa = WQ == kWUint8Group ? w.fa[WQ == kWUint8Group ? rt : 0] : 1.f;
-    const float fb = WQ == kWUint8Group ? w.fb[WQ == kWUint8Group ? rt : 0] : 1.f;
-    acc[0] = fmaf(d[0], fa, acc[0]);
-    acc[1] = fmaf(d[1], fa, acc[1]);
-    acc[2] = fmaf(d[2], fb, acc[2]);
-    acc[3] = fmaf(d[3], fb, acc[3]);
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int j = n ? 0 : 1; j < StreamStep<WQ>::NMMA; ++j)
+        stream_mma_16816(d, c, c, c, c, b[n][2 * j], b[n][2 * j + 1]);
+  }
+}
+
+// acc += weights of row tile rt x the step's activation chunks.  The step's sum starts at zero (or
+// at its bias) and is added in fp32, except (STEPS false) for fp16 weights: a tensor core truncates
+// what it adds to a large accumulator, which over a long K shows in fp32 results, not in fp16 ones.
+template <int WQ, int RT, bool STEPS, int N>
+__device__ __forceinline__ void stream_mma(const StreamA<WQ, RT>& w, int rt,
+                                           const uint32_t (&b)[N][StreamStep<WQ>::NB],
+                                           const float (&bias)[4], float (&acc)[4]) {
+  using S = StreamStep<WQ>;
+  if constexpr (WQ != kWFp16 || STEPS) {
+    float d[4];
+    const bool from = WQ == kWInt8PerChannel;
+    stream_mma_16816(d, w.a[rt][0], w.b[rt][0], w.a[rt][1], w.b[rt][1], b[0][0], b[0][1],
+                from ? bias[0] : 0.f, from ? bias[1] : 0.f, from ? bias[2] : 0.f,
+                from ? bias[3] : 0.f);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int j = n ? 0 : 1; j < S::NMMA; ++j)
+        stream_mma_16816(d, w.a[rt][2 * j], w.b[rt][2 * j], w.a[rt][2 * j + 1], w.b[rt][2 * j + 1],
+                  b[n][2 * j], b[n][2 * j + 1]);
+    if constexpr (WQ == kWUint8Group) {
+      acc[0] = fmaf(fmaf(-w.za[rt], bias[0], d[0]), w.fa[rt], acc[0]);
+      acc[1] = fmaf(fmaf(-w.za[rt], bias[1], d[1]), w.fa[rt], acc[1]);
+      acc[2] = fmaf(fmaf(-w.zb[rt], bias[0], d[2]), w.fb[rt], acc[2]);
+      acc[3] = fmaf(fmaf(-w.zb[rt], bias[1], d[3]), w.fb[rt], acc[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += d[i];
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < S::NMMA; ++j)
-      mma_16816(acc, w.a[rt][2 * j], w.b[rt][2 * j], w.a[rt][2 * j + 1], w.b[rt][2 * j + 1],
-                b[2 * j], b[2 * j + 1]);
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int j = 0; j < S::NMMA; ++j)
+        stream_mma_16816(acc, w.a[rt][2 * j], w.b[rt][2 * j], w.a[rt][2 * j + 1], w.b[rt][2 * j + 1],
+                  b[n][2 * j], b[n][2 * j + 1]);
   }
 }
 
-// How many of nsteps steps warp w of NW has: w, w + NW, ...
-template <int NW>
-__device__ __forceinline__ int stream_count(int warp, int nsteps) {
-  return nsteps > warp ? (nsteps - warp + NW - 1) / NW : 0;
+// [lo, hi) of part `id` of n items in `count` parts of sizes that differ by at most one.
+__device__ __forceinline__ void split_even(unsigned n, unsigned id, unsigned count, int& lo,
+                                           int& hi) {
+  const unsigned q = n / count, r = n - q * count;
+  lo = (int)(id * q + min(id, r));
+  hi = lo + (int)(q + (id < r ? 1u : 0u));
 }
 
-// The work of one CTA as a sequence of pieces (RT row tiles x all of K), streamed without a pause
-// between them: a warp's copies run S - 1 steps ahead of its arithmetic across piece boundaries,
-// so the next piece is in flight while this one's partial sums are added.
+// Worker `id` of `count`: this warp is its `warp`-th of `warps`.
+struct StreamWorker {
+  int id, count, in_cta, warp, warps;
+};
+template <int NW>
+__device__ __forceinline__ StreamWorker stream_worker(int ks) {
+  const int w = threadIdx.x >> 5, sh = 31 - __clz(ks);  // ks divides NW, both powers of two
+  const int per = NW >> sh;
+  return {(int)blockIdx.x * per + (w >> sh), (int)gridDim.x * per, w >> sh, w & (ks - 1), ks};
+}
+
+// The work of one worker -- KS warps of a CTA -- as a sequence of pieces (RT row tiles x all of K),
+// streamed without a pause between them: a warp's copies run S - 1 steps ahead of its arithmetic
+// across piece boundaries, so the next piece is in flight while this one's partial sums are added.
+// The warps of a worker split K (warp w: steps w, w + KS, ...); a CTA of NW warps has NW / KS
+// workers, which share nothing and meet at barriers of their own.  Fewer warps to a worker: more
+// steps to a piece, so less of its fixed cost (its sums' way through shared memory, its pointers);
+// more: fewer rows needed to fill the row tiles.
 //
-// Job::ROTATE: CTA b starts at step nsteps b / G and wraps around, so that CTAs that run together
-// read different k of the activations they share, not all of them the same few lines of L2 at once
-// (int8 M = 16: 26 us without, 21 with).  The order of a sum then depends on its CTA.
+// Job::ROTATE: worker b of G starts at step nsteps b / G and wraps around, so that workers that run
+// together read different k of the activations they share, not all of them the same few lines of
+// L2 at once (int8 M = 16: 26 us without, 21 with).  The order of a sum depends on its worker.
 //
 // Job: Piece, first(Piece&), next(Piece&) -> whether there is (another) piece;
-//      copy(piece, step, stage) issues one step; use_cols(piece) -> bit mg: the lane's column of
-//      group mg exists; live(piece) -> bit mg: any column of group mg exists (warp-uniform);
+//      copy(piece, step, stage) issues one step; live(piece) -> bit mg: any column of group mg
+//      exists (warp-uniform);
 //      z_rows(piece, r) the first row of each tile; finish(piece, rt, mg, float4) the whole sums
 //      of (row g, columns 2t, 2t + 1) and (row g + 8, the same).
 template <int WQ, int MG, int RT, int BV, int NW, int S, bool STEPS = false, class Job>
-__device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red, int nsteps) {
+__device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red_all, int nsteps,
+                                           StreamWorker wk) {
   using F = StreamFifo<WQ, MG, RT, BV>;
   using St = StreamStep<WQ>;
   static_assert(BV == St::NB / 4, "activations as they are");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t fifo = smem_u32(smem) + warp * S * F::STAGE;
+  const int lane = threadIdx.x & 31, warp = wk.warp, KS = wk.warps;
+  const uint8_t* fifo_p = smem + (threadIdx.x >> 5) * S * F::STAGE;
+  const uint32_t fifo = smem_u32(fifo_p);
+  float4* red = red_all + wk.in_cta * KS * RT * MG * 32;
   typename Job::Piece lp, up;
-  const int n_mine = stream_count<NW>(warp, nsteps);
+  const int n_mine = nsteps > warp ? ((nsteps - 1 - warp) >> (31 - __clz(KS))) + 1 : 0;
   bool more = n_mine > 0 && job.first(lp);
-  const int rot = Job::ROTATE ? (int)((long long)nsteps * blockIdx.x / gridDim.x) : 0;
+  const int rot = Job::ROTATE ? (int)((unsigned)(nsteps * wk.id) / (unsigned)wk.count) : 0;
   int lstep = warp, lslot = 0;
   auto issue = [&]() {
     if (more) {
       const int step = lstep + rot;
       job.copy(lp, step < nsteps ? step : step - nsteps, fifo + lslot * F::STAGE);
-      lstep += NW;
+      lstep += KS;
       if (lstep >= nsteps) {
         lstep = warp;
         more = job.next(lp);
@@ -264,65 +316,46 @@ __device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red,
     float acc[RT][MG][4] = {};
     int z_row[RT];
     job.z_rows(up, z_row);
-    const unsigned cols = job.use_cols(up), live = job.live(up);
+    const unsigned live = job.live(up);
 #pragma unroll 1
     for (int j = 0; j < n_mine; ++j) {
       cp_async_wait<S - 2>();
       __syncwarp();  // every lane's copies of this step; every lane is done with the previous one
       issue();
-      const uint32_t stage = fifo + slot * F::STAGE;
+      const uint8_t* stage = fifo_p + slot * F::STAGE;
       StreamA<WQ, RT> w;
       stream_read_weights<WQ, RT>(w, stage, F::Z_OFF, z_row, lane);
 #pragma unroll
       for (int mg = 0; mg < MG; ++mg) {
         if (MG > 1 && !((live >> mg) & 1u)) continue;
-        uint32_t b[St::NB];
+        uint32_t b[1][St::NB];
 #pragma unroll
         for (int v = 0; v < BV; ++v) {
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if ((cols >> mg) & 1u)
-            x = lds16(stage + F::B_OFF + b_vec<BV>(mg, BV * (lane & 3) + v, lane >> 2));
-          b[4 * v] = x.x;
-          b[4 * v + 1] = x.y;
-          b[4 * v + 2] = x.z;
-          b[4 * v + 3] = x.w;
+          // a column that does not exist holds whatever the FIFO held: it stays in its column
+          const uint4 x = lds16(stage + F::B_OFF + b_vec<BV>(mg, BV * (lane & 3) + v, lane >> 2));
+          b[0][4 * v] = x.x;
+          b[0][4 * v + 1] = x.y;
+          b[0][4 * v + 2] = x.z;
+          b[0][4 * v + 3] = x.w;
         }
+        float bias[4];
+        stream_bias<WQ>(b, bias);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) stream_mma<WQ, RT, STEPS>(w, rt, b, acc[rt][mg]);
+        for (int rt = 0; rt < RT; ++rt) stream_mma<WQ, RT, STEPS>(w, rt, b, bias, acc[rt][mg]);
       }
       slot = slot + 1 == S ? 0 : slot + 1;
     }
-    // the upper half of the warps hands its sums to the lower half, which adds its own
-    constexpr int HALF = NW > 8 ? NW / 2 : NW;
-    if (NW > 8 && warp >= HALF) {
 #pragma unroll
-      for (int i = 0; i < RT * MG; ++i) {
-        const float(&v)[4] = acc[i / MG][i % MG];
-        red[((warp - HALF) * RT * MG + i) * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
-      }
+    for (int i = 0; i < RT * MG; ++i) {
+      const float(&v)[4] = acc[i / MG][i % MG];
+      red[(warp * RT * MG + i) * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
     }
-    if (NW > 8) __syncthreads();
-    if (warp < HALF) {
-#pragma unroll
-      for (int i = 0; i < RT * MG; ++i) {
-        const float(&v)[4] = acc[i / MG][i % MG];
-        float4& r = red[(warp * RT * MG + i) * 32 + lane];
-        float4 o = make_float4(v[0], v[1], v[2], v[3]);
-        if (NW > 8) {
-          o.x += r.x;
-          o.y += r.y;
-          o.z += r.z;
-          o.w += r.w;
-        }
-        r = o;
-      }
-    }
-    __syncthreads();
-    // whole warps take whole (rt, mg) groups
-    for (int i = warp; i < RT * MG; i += NW) {
+    named_barrier_sync(1 + wk.in_cta, 32 * KS);
+    // whole warps take whole (rt, mg) groups, and add the warps' sums in order
+    for (int i = warp; i < RT * MG; i += KS) {
       float4 v = red[i * 32 + lane];
-#pragma unroll
-      for (int w = 1; w < HALF; ++w) {
+#pragma unroll 5
+      for (int w = 1; w < KS; ++w) {
         const float4 x = red[(w * RT * MG + i) * 32 + lane];
         v.x += x.x;
         v.y += x.y;
@@ -331,7 +364,7 @@ __device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red,
       }
       job.finish(up, i / MG, i % MG, v);
     }
-    __syncthreads();
+    named_barrier_sync(1 + wk.in_cta, 32 * KS);
   }
   cp_async_wait<0>();
 }
@@ -359,11 +392,18 @@ struct LinearJob {
   struct Piece {
     int i, n0, n1;
     const uint8_t* w;  // this lane's chunk of row n0 + g at k = 0
+    GroupWord z[WQ == kWUint8Group ? RT : 1];
   };
   __device__ __forceinline__ void bounds(Piece& p) const {
     p.n0 = lo + (hi - lo) * p.i / npieces;
     p.n1 = lo + (hi - lo) * (p.i + 1) / npieces;
     p.w = a.W + ((long long)(p.n0 + (lane >> 2)) * a.ldw + (lane & 3) * St::KC) * St::ESZ;
+    if (WQ == kWUint8Group) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        p.z[WQ == kWUint8Group ? rt : 0] =
+            group_word(a.scale, a.zero, p.n0 + rt * 16, a.N, lane);
+    }
   }
   __device__ __forceinline__ bool first(Piece& p) const {
     p.i = 0;
@@ -388,11 +428,9 @@ struct LinearJob {
       if (ra < p.n1) cp_async16(d, w, ok);
       if (ra + 8 < p.n1) cp_async16(d + 512, w + half, ok);
       w += 2 * half;
-      if (WQ == kWUint8Group) {
-        const long long gi = (long long)step_group(step, per_group) * a.N;
-        copy_group_row(stage + F::Z_OFF + rt * 128, a.scale + gi, a.zero + gi, p.n0 + rt * 16,
-                       a.N, lane, true);
-      }
+      if (WQ == kWUint8Group)
+        copy_group_word(stage + F::Z_OFF + rt * 128, p.z[WQ == kWUint8Group ? rt : 0],
+                        step_group(step, per_group), lane);
     }
 #pragma unroll
     for (int mg = 0; mg < MG; ++mg) {
@@ -405,12 +443,6 @@ struct LinearJob {
                      kw + 32 * v + 8 * (lane & 3) < a.K);
       }
     }
-  }
-  __device__ __forceinline__ unsigned use_cols(const Piece&) const {
-    unsigned c = 0;
-#pragma unroll
-    for (int mg = 0; mg < MG; ++mg) c |= (mg * 8 + (lane >> 2) < a.M ? 1u : 0u) << mg;
-    return c;
   }
   __device__ __forceinline__ unsigned live(const Piece&) const { return (1u << MG) - 1u; }
   __device__ __forceinline__ void z_rows(const Piece& p, int (&r)[RT]) const {
@@ -431,14 +463,14 @@ struct LinearJob {
   }
 };
 
-// NW warps share the shared memory left beside the partial sums.  16 of them: with 8 the unpacking
-// of 8-bit weights ran at the speed of two warps per scheduler, not of the memory.
+// 16 warps share the shared memory left beside the partial sums: with 8 the unpacking of 8-bit
+// weights ran at the speed of two warps per scheduler, not of the memory.
 template <int WQ, int MG, int RT>
 struct LinearCfg {
-  static constexpr int NW = LIN_NW;
+  static constexpr int NW = 16;
   static constexpr int BV = StreamStep<WQ>::NB / 4;
   using F = StreamFifo<WQ, MG, RT, BV>;
-  static constexpr int RED = 8 * RT * MG * 512;
+  static constexpr int RED = NW * RT * MG * 512;
   static constexpr int S = F::depth((kMaxDynSmem - RED) / NW);
   static constexpr int FIFO = NW * S * F::STAGE;
   static constexpr int SMEM = FIFO + RED;
@@ -447,21 +479,21 @@ struct LinearCfg {
 
 template <int WQ, int MG, int RT>
 __global__ void __launch_bounds__(32 * LinearCfg<WQ, MG, RT>::NW, 1)
-    k_stream_linear(const LinearArgs a) {
+    k_stream_linear(const LinearArgs a, int ks) {
   using C = LinearCfg<WQ, MG, RT>;
   extern __shared__ __align__(16) uint8_t smem[];
   pdl_wait();
   pdl_launch_dependents();
+  const StreamWorker wk = stream_worker<C::NW>(ks);
   LinearJob<WQ, MG, RT> job{a};
-  job.lo = (int)((long long)a.N * blockIdx.x / gridDim.x);
-  job.hi = (int)((long long)a.N * (blockIdx.x + 1) / gridDim.x);
+  split_even(a.N, wk.id, wk.count, job.lo, job.hi);
   job.npieces = (job.hi - job.lo + 16 * RT - 1) / (16 * RT);
   job.lane = threadIdx.x & 31;
   job.per_group = group_magic<WQ>(a.group);
   job.x = a.A + (job.lane >> 2) * a.lda + 8 * (job.lane & 3);
   stream_run<WQ, MG, RT, C::BV, C::NW, C::S>(
       job, smem, reinterpret_cast<float4*>(smem + C::FIFO),
-      (a.K + StreamStep<WQ>::STEP - 1) / StreamStep<WQ>::STEP);
+      (a.K + StreamStep<WQ>::STEP - 1) / StreamStep<WQ>::STEP, wk);
 }
 
 }  // namespace tempo_sm100
