@@ -48,6 +48,7 @@ EXPORTS = {
     "tempo_sm100_gemm_fp16_swiglu": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "tempo_sm100_gemm_w8a16_swiglu": (
         _i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "tempo_sm100_epilogue_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "tempo_sm100_gemm_fp16_epilogue": (_i, [_vp] * 5 + [_i] * 8 + [_vp, _sz, _vp]),
     "tempo_sm100_gemm_w8a16_epilogue": (_i, [_vp] * 7 + [_i] * 10 + [_vp, _sz, _vp]),
     "tempo_sm100_moe_route": (_i, [_vp] * 5 + [_i] * 7 + [_vp]),

@@ -1,13 +1,15 @@
 // The GEMM with a fused epilogue, y = act(A W^T + bias) + residual: which kernel runs.
 //
 //   M <= 16    k_stream_linear (stream.cuh)
-//   M > 16     the hyperform the shipped dispatcher plans for the same problem, in its EPI
-//              instantiation; W8A16 at prefill sizes expands the weights to fp16 first, the
-//              per-channel kind without its scale, which multiplies the fp32 accumulator instead
-//              (an int8 value is exact in fp16, its product with a scale is not).
+//   M <= 384   k_epi_swap (swap_tile.cuh); 8-bit weights up to 1279 rows
+//   above      the 2-CTA tiles the shipped dispatcher plans for the fp16 problem, with the epilogue
+//              on the accumulator; 8-bit weights are expanded to fp16 first, the per-channel kind
+//              without its scale, which multiplies the fp32 accumulator instead (an int8 value is
+//              exact in fp16, its product with a scale is not).
 #pragma once
 
 #include "stream.h"
+#include "swap_tile.cuh"
 
 namespace tempo_sm100 {
 
@@ -31,37 +33,22 @@ __global__ void __launch_bounds__(256)
 
 namespace {
 
+// Above kStreamMaxM rows: the swapped tiles, or the 2-CTA ones (8-bit weights expanded first).
+// Measured, swapped / 2-CTA us: fp16 400 x 3840 x 4096 31 / 36, 512 x 8192 x 3840 61 / 41,
+// 1024 x 15360 x 3840 186 / 106; 8-bit 512 x 10240 x 5120 91 / 93, 1024 x 5120 x 8192 97 / 118,
+// 1536 x 5120 x 17408 304 / 265, 4096 x 15360 x 3840 560 / 361.
+bool swap_epilogue(int M, int N, int K, int wkind, size_t ws_bytes) {
+  if (wkind == kWFp16) return M <= kSwapMaxRows;
+  return M < 1280 || ws_bytes < kExpandOffset + expand_ws_bytes(N, K);
+}
+
 cudaError_t run_pair_epi(const Problem& pr, const Hyper& h, cudaStream_t st) {
-  if (pr.wkind == kWInt8PerChannel)
-    return h.bn == 256 ? launch_pair_w8<256, 1, true>(pr, h, st)
-                       : launch_pair_w8<128, 1, true>(pr, h, st);
-  if (pr.wkind == kWUint8Group)
-    return h.bn == 256 ? launch_pair_w8<256, 2, true>(pr, h, st)
-                       : launch_pair_w8<128, 2, true>(pr, h, st);
   switch (h.bn) {
     case 256: return launch_pair<256, false, true>(pr, h, st);
     case 224: return launch_pair<224, false, true>(pr, h, st);
     case 192: return launch_pair<192, false, true>(pr, h, st);
     case 160: return launch_pair<160, false, true>(pr, h, st);
     case 128: return launch_pair<128, false, true>(pr, h, st);
-    default: return cudaErrorInvalidConfiguration;
-  }
-}
-
-// The EPI instantiations of the 1-CTA tiles the shipped ladders name from M = 17 on.
-cudaError_t run_tile_epi(const Problem& pr, const Hyper& h, cudaStream_t st) {
-  const int key = pr.wkind * 10000 + h.swap * 1000 + h.bn;
-  switch (key) {
-    case 1064: return launch_inst<64, 0, true, false, true>(pr, h, st);
-    case 1128: return launch_inst<128, 0, true, false, true>(pr, h, st);
-    case 128: return launch_inst<128, 0, false, false, true>(pr, h, st);
-    case 256: return launch_inst<256, 0, false, false, true>(pr, h, st);
-    case 12032: return launch_inst<32, 1, true, true, true>(pr, h, st);
-    case 12064: return launch_inst<64, 1, true, true, true>(pr, h, st);
-    case 11128: return launch_inst<128, 1, true, false, true>(pr, h, st);
-    case 22032: return launch_inst<32, 2, true, true, true>(pr, h, st);
-    case 22064: return launch_inst<64, 2, true, true, true>(pr, h, st);
-    case 21128: return launch_inst<128, 2, true, false, true>(pr, h, st);
     default: return cudaErrorInvalidConfiguration;
   }
 }
@@ -73,27 +60,25 @@ cudaError_t run_epilogue(const Problem& pr, cudaStream_t st) {
                        static_cast<__half*>(pr.C), pr.epi, pr.M, pr.N, pr.K, pr.lda, pr.ldw,
                        pr.ldc, pr.group > 0 ? pr.group : 1},
                       pr.wkind, st);
+  if (swap_epilogue(pr.M, pr.N, pr.K, pr.wkind, pr.ws ? pr.ws_bytes : 0)) {
+    switch (pr.wkind) {
+      case kWFp16: return launch_epi_swap<kWFp16>(pr, st);
+      case kWInt8PerChannel: return launch_epi_swap<kWInt8PerChannel>(pr, st);
+      default: return launch_epi_swap<kWUint8Group>(pr, st);
+    }
+  }
   const size_t cap = pr.ws ? pr.ws_bytes : 0;
   tempo::gen::Choice c{};
-  cudaError_t e;
-  if (pr.wkind == kWFp16) {
-    tempo::gen::GemmParams p{};
-    p.M = pr.M; p.N = pr.N; p.K = pr.K;
-    p.lda = (int)pr.lda; p.ldb = (int)pr.ldw; p.ldc = (int)pr.ldc;
-    p.ws_bytes = cap;
-    e = tempo::gen::plan(p, &c);
-  } else {
-    tempo::gen::W8A16Params p{};
-    p.M = pr.M; p.N = pr.N; p.K = pr.K;
-    p.lda = (int)pr.lda; p.ldw = (int)pr.ldw; p.ldc = (int)pr.ldc;
-    p.scale_kind = pr.wkind; p.group = pr.group;
-    p.ws_bytes = cap;
-    e = tempo::gen::plan(p, &c);
-  }
+  tempo::gen::GemmParams p{};
+  p.M = pr.M; p.N = pr.N; p.K = pr.K;
+  p.lda = (int)pr.lda; p.ldb = (int)pr.ldw; p.ldc = (int)pr.ldc;
+  p.ws_bytes = pr.wkind == kWFp16 ? cap : cap - expand_ws_bytes(pr.N, pr.K);
+  cudaError_t e = tempo::gen::plan(p, &c);
   if (e != cudaSuccess) return e;
+  if (c.cta_group != 2) return cudaErrorInvalidConfiguration;
   Hyper h{c.bn, c.swap, c.splits, c.group_m, 0};
   h.cta_group = c.cta_group;
-  if (c.expand) {
+  if (pr.wkind != kWFp16) {
     const size_t wexp = expand_ws_bytes(pr.N, pr.K);
     char* base = static_cast<char*>(pr.ws);
     __half* wf = reinterpret_cast<__half*>(base + kExpandOffset);
@@ -116,7 +101,16 @@ cudaError_t run_epilogue(const Problem& pr, cudaStream_t st) {
     q.ws_parts = base + kExpandOffset + wexp;
     return run_pair_epi(q, h, st);
   }
-  return c.cta_group == 2 ? run_pair_epi(pr, h, st) : run_tile_epi(pr, h, st);
+  return run_pair_epi(pr, h, st);
+}
+
+// Workspace run_epilogue would like (0: none).
+size_t epilogue_ws_bytes(int M, int N, int K, int wkind) {
+  if (M <= kStreamMaxM) return 0;
+  if (swap_epilogue(M, N, K, wkind, ~(size_t)0))
+    return epi_swap_plan(wkind, M, N, K, std::max(1, current_sms()), ~(size_t)0).ws_bytes;
+  const size_t ws = tempo_sm100_workspace_bytes(M, N, K, 0);
+  return wkind == kWFp16 ? ws : std::max(ws, (size_t)kExpandOffset) + expand_ws_bytes(N, K);
 }
 
 }  // namespace

@@ -245,6 +245,11 @@ int tempo_sm100_gemm_w8a16_swiglu(const void* A, const void* W, const void* scal
   return run_pair_swiglu(pr, current_sms(), st);
 }
 
+size_t tempo_sm100_epilogue_workspace_bytes(int M, int N, int K, int weight_kind) {
+  if (M < 1 || N < 1 || K < 1 || weight_kind < 0 || weight_kind > 2) return 0;
+  return epilogue_ws_bytes(M, N, K, weight_kind);
+}
+
 int tempo_sm100_gemm_fp16_epilogue(const void* A, const void* B, void* C, const void* bias,
                                    const void* residual, int M, int N, int K, int lda, int ldb,
                                    int ldc, int ldr, int activation, void* ws, size_t ws_bytes,

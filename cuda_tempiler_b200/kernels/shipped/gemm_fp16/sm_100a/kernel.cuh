@@ -506,7 +506,7 @@ namespace tempo_sm100 {
 
 enum WeightQuant : int { kWFp16 = 0, kWInt8PerChannel = 1, kWUint8Group = 2 };
 
-// Epilogue of the EPI instantiations: y = act(acc * scale[n] + bias[n]) + res[m][n], in fp32 on
+// Epilogue of the 2-CTA kernels' EPI instantiations: y = act(acc * scale[n] + bias[n]) + res[m][n], in fp32 on
 // the accumulator, rounded once to fp16.  Null pointers leave their term out.  Every load is 16
 // bytes of 8 columns (N % 8 == 0, 16-byte aligned), made where the accumulator already is: the
 // separate pass it replaces reads and writes C once more (4 M N bytes).
@@ -686,8 +686,8 @@ __device__ __forceinline__ float epi_act(float x, int act) {
     case kActRelu: return x > 0.f || x != x ? x : 0.f;  // NaN passes through
     case kActSilu: return x / (1.f + expf(-x));
     case kActGelu: return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-    case kActGeluTanh:
-      return 0.5f * x * (1.f + tanhf(0.79788456080286536f * (x + 0.044715f * x * x * x)));
+    case kActGeluTanh:  // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)): one exponential, one division
+      return x / (1.f + expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
     default: return x;
   }
 }
@@ -702,10 +702,24 @@ __device__ __forceinline__ void unpack_half8(uint4 v, float (&f)[8]) {
   }
 }
 
-// The epilogue of columns [n0, n0 + 32) of row m held by one thread.  The residual is read with
-// plain loads: C may be the same memory, and this thread reads an element before anyone writes it.
-__device__ __forceinline__ void epi_row32(const EpiArgs& e, float (&f)[32], int m, int m_rows,
-                                          int n0, int n_cols) {
+// Columns [n0, n0 + 32) of the residual's row m, for one thread, loaded while an earlier chunk is
+// worked on, or before the tile's MMAs are done (4096 x 3840 x 15360 with the loads where the values
+// are added: 397 us, so: 378).  Plain loads: C may be the same memory, and this thread reads an
+// element before anyone writes it.
+struct EpiRes {
+  uint4 v[4];
+  __device__ __forceinline__ void load(const EpiArgs& e, int m, int m_rows, int n0, int n_cols) {
+    if (!e.res || m >= m_rows) return;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (n0 + 8 * g < n_cols)
+        v[g] = *reinterpret_cast<const uint4*>(e.res + (long long)m * e.ldr + n0 + 8 * g);
+  }
+};
+
+// The epilogue of columns [n0, n0 + 32) of row m held by one thread.
+__device__ __forceinline__ void epi_row32(const EpiArgs& e, float (&f)[32], const EpiRes& res,
+                                          int m, int m_rows, int n0, int n_cols) {
   if (m >= m_rows) return;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
@@ -727,7 +741,7 @@ __device__ __forceinline__ void epi_row32(const EpiArgs& e, float (&f)[32], int 
       for (int i = 0; i < 8; ++i) f[8 * g + i] = epi_act(f[8 * g + i], e.act);
     }
     if (e.res) {
-      unpack_half8(*reinterpret_cast<const uint4*>(e.res + (long long)m * e.ldr + n), v);
+      unpack_half8(res.v[g], v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[8 * g + i] += v[i];
     }
@@ -741,7 +755,7 @@ __device__ __forceinline__ float epi_one(const EpiArgs& e, float v, float b, int
   return v;
 }
 
-template <int BN, int WQ, bool SWAP, bool SMEMDQ = false, bool EPI = false>
+template <int BN, int WQ, bool SWAP, bool SMEMDQ = false>
 __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
     k_gemm_sm100(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                  const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapC,
@@ -1108,17 +1122,6 @@ __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
               acc.z *= __half2float(__ldg(args.scale + n + 2));
               acc.w *= __half2float(__ldg(args.scale + n + 3));
             }
-            if (EPI) {
-              float b[4] = {0.f, 0.f, 0.f, 0.f};
-              if (args.epi.bias) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) b[i] = __half2float(__ldg(args.epi.bias + n + i));
-              }
-              acc.x = epi_one(args.epi, acc.x, b[0], m, n);
-              acc.y = epi_one(args.epi, acc.y, b[1], m, n + 1);
-              acc.z = epi_one(args.epi, acc.z, b[2], m, n + 2);
-              acc.w = epi_one(args.epi, acc.w, b[3], m, n + 3);
-            }
             uint2 w;
             w.x = pack_half2(acc.x, acc.y);
             w.y = pack_half2(acc.z, acc.w);
@@ -1158,7 +1161,6 @@ __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
               f[j] *= __half2float(q < args.weight_rows ? __ldg(args.scale + q) : __half(0.f));
             }
           }
-          if (EPI) epi_row32(args.epi, f, p, args.rows_p, q0 + c * 32, args.rows_q);
           if (lane == 0) bulk_wait_group_read<1>();
           __syncwarp();
           uint8_t* sbuf = stage_buf + sb * 2048;
@@ -1184,8 +1186,6 @@ __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
         // swapped: C[q][p]; lanes run along p (= n), so each column store is coalesced.
         const float sc =
             (WQ == kWInt8PerChannel && p < args.rows_p) ? __half2float(__ldg(args.scale + p)) : 1.f;
-        const float bias = (EPI && args.epi.bias && p < args.rows_p)
-                               ? __half2float(__ldg(args.epi.bias + p)) : 0.f;
 #pragma unroll 1
         for (int c = 0; c < BN / Cfg::CW; ++c) {
           float f[32];
@@ -1199,11 +1199,8 @@ __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
 #pragma unroll
             for (int j = 0; j < Cfg::CW; ++j) {
               const int q = q0 + c * Cfg::CW + j;
-              if (q < args.rows_q) {
-                float v = f[j] * sc;
-                if (EPI) v = epi_one(args.epi, v, bias, q, p);
-                args.C[(long long)q * args.ldc + p] = __float2half_rn(v);
-              }
+              if (q < args.rows_q)
+                args.C[(long long)q * args.ldc + p] = __float2half_rn(f[j] * sc);
             }
           }
         }
@@ -2119,11 +2116,13 @@ __global__ void __launch_bounds__(PairCfg<BN>::THREADS, 1)
       tile_pos(args, sg.tile, tp, tq);
       const int buf = lu & 1;
       const uint32_t uphase = (lu >> 1) & 1;
+      const int q0 = tq * BN;
+      const int row0 = tp * 256 + (int)rank * 128 + quad * 32;
+      EpiRes res;
+      if (EPI && sg.contrib <= 1) res.load(args.epi, row0 + lane, args.rows_p, q0, args.rows_q);
       if (!mbar_wait(tfull_bar(buf), uphase, abort_flag, 14)) break;
       tc_fence_after();
       const uint32_t t_acc = t_lane + buf * Cfg::ACC_STRIDE;
-      const int q0 = tq * BN;
-      const int row0 = tp * 256 + (int)rank * 128 + quad * 32;
       if (sg.contrib > 1 && (args.ws == nullptr || args.counters == nullptr)) {
         // a tail without workspace is a host-side bug: report it instead of faulting
         if (lane == 0 && atomicCAS(&g_status[0], 0, 2) == 0) {
@@ -2177,6 +2176,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::THREADS, 1)
         const int S = sg.contrib;
 #pragma unroll 1
         for (int c = 0; c < BN / 32; ++c) {
+          if (EPI) res.load(args.epi, p, args.rows_p, q0 + c * 32, args.rows_q);
           float acc[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[i] = 0.f;
@@ -2220,7 +2220,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::THREADS, 1)
             if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(buf), 0));
           }
           if (p >= args.rows_p) continue;
-          if (EPI) epi_row32(args.epi, acc, p, args.rows_p, q0 + c * 32, args.rows_q);
+          if (EPI) epi_row32(args.epi, acc, res, p, args.rows_p, q0 + c * 32, args.rows_q);
 #pragma unroll
           for (int i0 = 0; i0 < 32; i0 += 8) {
             const int q = q0 + c * 32 + i0;
@@ -2293,7 +2293,12 @@ __global__ void __launch_bounds__(PairCfg<BN>::THREADS, 1)
           if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(buf), 0));
         }
         if (!rows_live) continue;
-        if (EPI) epi_row32(args.epi, f, row0 + lane, args.rows_p, q0 + c * 32, args.rows_q);
+        if (EPI) {
+          const EpiRes cur = res;
+          if (c + 1 < nchunk)
+            res.load(args.epi, row0 + lane, args.rows_p, q0 + c * 32 + 32, args.rows_q);
+          epi_row32(args.epi, f, cur, row0 + lane, args.rows_p, q0 + c * 32, args.rows_q);
+        }
         if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
         uint8_t* sbuf = stage_buf + sb * 2048;
@@ -2384,7 +2389,7 @@ struct PairW8Cfg {
   static_assert(SMEM <= kMaxDynSmem, "shared memory");
 };
 
-template <int BN, int WQ, bool EPI = false>
+template <int BN, int WQ>
 __global__ void __launch_bounds__(PairW8Cfg<BN>::THREADS, 1)
     k_gemm_sm100_pair_w8(const __grid_constant__ CUtensorMap mapA,
                          const __grid_constant__ CUtensorMap mapW,
@@ -2734,13 +2739,11 @@ __global__ void __launch_bounds__(PairW8Cfg<BN>::THREADS, 1)
             if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(buf), 0));
           }
           if (p >= args.rows_p) continue;
-          // EPI instantiations take the per-channel scale as epi.scale
-          if (EPI) epi_row32(args.epi, acc, p, args.rows_p, q0 + c * 32, args.rows_q);
 #pragma unroll
           for (int i0 = 0; i0 < 32; i0 += 8) {
             const int q = q0 + c * 32 + i0;
             if (q >= args.rows_q) break;
-            if (WQ == kWInt8PerChannel && !EPI) {
+            if (WQ == kWInt8PerChannel) {
 #pragma unroll
               for (int j = 0; j < 8; ++j)
                 acc[i0 + j] *= q + j < args.rows_q ? __half2float(__ldg(args.scale + q + j)) : 0.f;
@@ -2762,7 +2765,7 @@ __global__ void __launch_bounds__(PairW8Cfg<BN>::THREADS, 1)
       for (int c = 0; c < nchunk; ++c) {
         float f[32];
         acc_chunk<32, 1, BN>(t_acc, c, f);
-        if (WQ == kWInt8PerChannel && !EPI) {
+        if (WQ == kWInt8PerChannel) {
           // per-output-channel scale of columns q0 + 32 c + j: lane j loads one, all share it
           const int n = q0 + c * 32 + lane;
           const float sv = n < args.rows_q ? __half2float(__ldg(args.scale + n)) : 0.f;
@@ -2775,7 +2778,6 @@ __global__ void __launch_bounds__(PairW8Cfg<BN>::THREADS, 1)
           if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(buf), 0));
         }
         if (!rows_live) continue;
-        if (EPI) epi_row32(args.epi, f, row0 + lane, args.rows_p, q0 + c * 32, args.rows_q);
         if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
         uint8_t* sbuf = stage_buf + sb * 2048;

@@ -216,12 +216,10 @@ size_t ws_needed(int tiles, int splits, int bn) {
 // ------------------------------------------------------------------------------------------
 // Instantiation table.
 // ------------------------------------------------------------------------------------------
-// EPI: the instantiation with the fused epilogue (k-splits through the global workspace have none).
-template <int BN, int WQ, bool SWAP, bool SMEMDQ = false, bool EPI = false>
+template <int BN, int WQ, bool SWAP, bool SMEMDQ = false>
 cudaError_t launch_inst(const Problem& pr, const Hyper& h, cudaStream_t st) {
   using Cfg = SkelCfg<BN, WQ, SWAP, SMEMDQ>;
-  auto kern = k_gemm_sm100<BN, WQ, SWAP, SMEMDQ, EPI>;
-  if (EPI && h.splits > kMaxClusterSplit) return cudaErrorInvalidConfiguration;
+  auto kern = k_gemm_sm100<BN, WQ, SWAP, SMEMDQ>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -264,7 +262,6 @@ cudaError_t launch_inst(const Problem& pr, const Hyper& h, cudaStream_t st) {
   a.group_size = pr.group > 0 ? pr.group : 1;
   a.groups_per_row = pr.group > 0 ? pr.K / pr.group : 1;
   a.weight_rows = pr.N;
-  if (EPI) a.epi = pr.epi;
 
   CUtensorMap mP, mQ, mW, mC, mS, mZ;
   std::memset(&mS, 0, sizeof(mS));
@@ -606,10 +603,10 @@ cudaError_t launch_pair(const Problem& pr, const Hyper& h, cudaStream_t st) {
 
 // W8A16 2-CTA launch (k_gemm_sm100_pair_w8): persistent clusters; h.splits > 1 allows the
 // split tail of pair_plan (given the workspace it needs).
-template <int BN, int WQ, bool EPI = false>
+template <int BN, int WQ>
 cudaError_t launch_pair_w8(const Problem& pr, const Hyper& h, cudaStream_t st) {
   using Cfg = PairW8Cfg<BN>;
-  auto kern = k_gemm_sm100_pair_w8<BN, WQ, EPI>;
+  auto kern = k_gemm_sm100_pair_w8<BN, WQ>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -645,10 +642,6 @@ cudaError_t launch_pair_w8(const Problem& pr, const Hyper& h, cudaStream_t st) {
   a.zero = static_cast<const uint8_t*>(pr.zero);
   a.group_size = pr.group > 0 ? pr.group : 1;
   a.groups_per_row = pr.group > 0 ? pr.K / pr.group : 1;
-  if (EPI) {
-    a.epi = pr.epi;
-    if (WQ == kWInt8PerChannel) a.epi.scale = static_cast<const __half*>(pr.scale);
-  }
   a.sk_tile0 = pl.sk_tile0;
   a.sk_tiles = pl.sk_tiles;
   a.sk_splits = pl.sk_splits;

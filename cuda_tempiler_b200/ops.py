@@ -327,7 +327,7 @@ def gemm_fp16_epilogue(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | No
             out = torch.empty((M, N), dtype=torch.float16, device=dev)
         ws = None
         if M > STREAM_MAX_M:
-            ws = _call_workspace(dev, lib.tempo_sm100_workspace_bytes(M, N, K, 0))
+            ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, 0))
         rc = lib.tempo_sm100_gemm_fp16_epilogue(
             A.data_ptr(), B.data_ptr(), out.data_ptr(), _ptr(bias), _ptr(residual), M, N, K,
             A.stride(0), B.stride(0), out.stride(0), ldr, act, _ptr(ws),
@@ -382,7 +382,7 @@ def gemm_w8a16_epilogue(A: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
             out = torch.empty((M, N), dtype=torch.float16, device=dev)
         ws = None
         if M > STREAM_MAX_M:
-            ws = _call_workspace(dev, lib.tempo_sm100_workspace_bytes(M, N, K, kind))
+            ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, kind))
         rc = lib.tempo_sm100_gemm_w8a16_epilogue(
             A.data_ptr(), W.data_ptr(), scale.data_ptr(), _ptr(zero), out.data_ptr(), _ptr(bias),
             _ptr(residual), M, N, K, A.stride(0), W.stride(0), out.stride(0), ldr, kind,

@@ -54,10 +54,7 @@ def parse_ptxas(log: str) -> dict:
 
 
 def demangle_family(mangled: str) -> str | None:
-    """'_ZN11tempo_sm10012k_gemm_sm100ILi256ELi0ELb0EEEv...' -> 'tempo_sm100::k_gemm_sm100<256, 0, false>'.
-    The instantiations with a fused epilogue (fifth parameter true) are not search-space points."""
-    if re.search(r"k_gemm_sm100ILi\d+ELi\d+ELb[01]ELb[01]ELb1E", mangled):
-        return None
+    """'_ZN11tempo_sm10012k_gemm_sm100ILi256ELi0ELb0EEEv...' -> 'tempo_sm100::k_gemm_sm100<256, 0, false>'."""
     m = re.search(r"k_gemm_sm100ILi(\d+)ELi(\d+)ELb([01])E", mangled)
     if not m:
         return None

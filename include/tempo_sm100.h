@@ -144,7 +144,9 @@ int tempo_sm100_gemm_w8a16_swiglu(const void* A, const void* W, const void* scal
 
 /* GEMM with a fused epilogue: C = act(A W^T + bias) + residual, the epilogue in fp32 on the
  * accumulator and one rounding to fp16.  Layouts, strides, coverage and return codes of
- * tempo_sm100_gemm_fp16 / tempo_sm100_gemm_w8a16; workspace as tempo_sm100_workspace_bytes says.
+ * tempo_sm100_gemm_fp16 / tempo_sm100_gemm_w8a16; workspace as
+ * tempo_sm100_epilogue_workspace_bytes says (zero-filled once like the GEMMs', and interchangeable
+ * with theirs; NULL runs without).
  * bias: fp16 [N] or NULL.  residual: fp16 [M][N], row stride ldr elements, or NULL; it may be C
  * itself (same pointer and stride), no other overlap.  bias, residual and (W8A16) scale 16-byte
  * aligned, ldr a multiple of 8 (else 9).  activation: a TEMPO_ACT_* value (else 1). */
@@ -153,6 +155,7 @@ int tempo_sm100_gemm_w8a16_swiglu(const void* A, const void* W, const void* scal
 #define TEMPO_ACT_SILU 2
 #define TEMPO_ACT_GELU 3       /* x Phi(x) */
 #define TEMPO_ACT_GELU_TANH 4  /* its tanh approximation */
+size_t tempo_sm100_epilogue_workspace_bytes(int M, int N, int K, int weight_kind);
 int tempo_sm100_gemm_fp16_epilogue(const void* A, const void* B, void* C, const void* bias,
                                    const void* residual, int M, int N, int K, int lda, int ldb,
                                    int ldc, int ldr, int activation, void* ws, size_t ws_bytes,

@@ -1,6 +1,6 @@
 """GPU parity of the GEMM with a fused epilogue against its 64-bit restatement: every path (the
-weight stream, the 1-CTA tiles with and without a k-split, the 2-CTA tiles with and without a
-split tail, the expanded prefill), every activation, ragged sizes, strides, in-place residuals."""
+weight stream, the swapped tiles whole and in shares, the 2-CTA tiles with and without a split
+tail, the expanded prefill), every activation, ragged sizes, strides, in-place residuals."""
 import itertools
 
 import pytest
@@ -113,6 +113,20 @@ def test_split_tail(dev, M, N, K):
     bias, res = rand(N, seed=6), rand(M, N, seed=7)
     for _ in range(2):
         check(call(A, w, 0, bias=bias, activation="relu", residual=res), A, w, 0, bias, "relu", res)
+
+
+@pytest.mark.parametrize("kind,group", [("fp16", 0), ("int8", 0), ("uint8", 128)])
+@pytest.mark.parametrize("M", [16, 17, 100, 256, 257, 340, 384, 385, 512, 768, 769, 1100, 1279, 1280])
+@pytest.mark.parametrize("N,K", [(3840, 2048), (528, 8192)])
+def test_long_shares(dev, kind, group, M, N, K):
+    """Rows around every edge of the dispatch, k ranges that go round each ring of buffers often:
+    right, and the same in every run."""
+    A, w = rand(M, K, seed=M), weights(kind, N, K, group, seed=5)
+    res = rand(M, N, seed=6)
+    y = call(A, w, group, residual=res)
+    check(y, A, w, group, None, "none", res)
+    for _ in range(5):
+        assert torch.equal(y, call(A, w, group, residual=res))
 
 
 @pytest.mark.parametrize("kind,group", [("fp16", 0), ("int8", 0), ("uint8", 64)])
