@@ -88,6 +88,8 @@ class NotCovered(RuntimeError):
 def load(path: Path | str | None = None, build_if_missing: bool = True) -> C.CDLL:
     """Load (building first if absent or stale and nvcc exists) and bind every export."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

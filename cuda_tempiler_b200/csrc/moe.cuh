@@ -202,14 +202,14 @@ struct RouteArgs {
   MoePlan* plan;
 };
 
-// The experts [lo, hi) times the tokens [t0, t0 + nt), 16 experts at a time.
+// The experts [lo, hi) times the nt tokens, 16 experts at a time.
 template <int MG>
 struct RouteJob {
   using St = StreamStep<kWFp16>;
   using F = StreamFifo<kWFp16, MG, 1, 1>;
   static constexpr bool ROTATE = false;  // equal router rows have equal logits
   const RouteArgs& a;
-  int lo, hi, t0, nt, lane;
+  int lo, hi, nt, lane;
   float* logits;  // [tokens this CTA owns][kMoeMaxE], the same place in every CTA of the cluster
   struct Piece {
     int n0;
@@ -232,7 +232,7 @@ struct RouteJob {
       const int m = mg * 8 + g;
       if (m < nt)
         cp_async16(stage + F::B_OFF + mg * 512 + lane * 16,
-                   a.x + (long long)(t0 + m) * a.ldx + kw + 8 * (lane & 3), ok);
+                   a.x + m * a.ldx + kw + 8 * (lane & 3), ok);
     }
   }
   __device__ __forceinline__ unsigned live(const Piece&) const {
@@ -267,10 +267,10 @@ struct RouteCfg {
   static constexpr int SMEM = FIFO + RED + REST;
 };
 
-// One cluster of 16 CTAs routes 8 or 32 tokens: CTA r multiplies them with the experts
+// One cluster of 16 CTAs routes up to 8 or 32 tokens: CTA r multiplies them with the experts
 // [E r / 16, E (r + 1) / 16) -- its share of the router's weights is in flight at once -- hands
 // each token's logits to the CTA that owns the token (t % 16) through distributed shared memory,
-// and picks the top-k of its own tokens, a warp each.  With a plan wanted (one cluster, T <= 32)
+// and picks the top-k of its own tokens, a warp each.  With a plan wanted
 // CTA 0 collects the choices and builds it.
 template <int MG>
 __global__ void __launch_bounds__(32 * RouteCfg<MG>::NW, 1) k_moe_route(const RouteArgs a) {
@@ -283,12 +283,11 @@ __global__ void __launch_bounds__(32 * RouteCfg<MG>::NW, 1) k_moe_route(const Ro
   int* ebase = reinterpret_cast<int*>(emask + kMoeMaxE);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = (int)cluster_ctarank();
-  const int t0 = (blockIdx.x / kRouteCluster) * C::TOK;
-  const int nt = min(C::TOK, a.T - t0);
+  const int nt = a.T;
   cluster_sync();  // every CTA of the cluster runs before its shared memory is written
   pdl_wait();
   pdl_launch_dependents();
-  RouteJob<MG> job{a, a.E * rank / kRouteCluster, a.E * (rank + 1) / kRouteCluster, t0, nt, lane,
+  RouteJob<MG> job{a, a.E * rank / kRouteCluster, a.E * (rank + 1) / kRouteCluster, nt, lane,
                    logits};
   stream_run<kWFp16, MG, 1, 1, C::NW, C::S, true>(
       job, smem, reinterpret_cast<float4*>(smem + C::FIFO),
@@ -297,8 +296,8 @@ __global__ void __launch_bounds__(32 * RouteCfg<MG>::NW, 1) k_moe_route(const Ro
   for (int q = warp; q < C::OWN; q += C::NW) {
     const int m = q * kRouteCluster + rank;
     if (m >= nt) continue;
-    int* id = a.ids + (long long)(t0 + m) * a.k;
-    float* w = a.weights + (long long)(t0 + m) * a.k;
+    int* id = a.ids + m * a.k;
+    float* w = a.weights + m * a.k;
     moe_topk(logits + q * kMoeMaxE, a.E, a.k, a.normalize != 0, id, w);
     if (a.plan && lane < a.k) {  // this lane wrote these two itself
       st_dsmem_f32(mapa_shared(smem_u32(s_ids + m * a.k + lane), 0), __int_as_float(id[lane]));
@@ -308,6 +307,147 @@ __global__ void __launch_bounds__(32 * RouteCfg<MG>::NW, 1) k_moe_route(const Ro
   if (!a.plan) return;
   cluster_sync();
   if (rank == 0) moe_build_plan(a.plan, s_ids, s_w, a.T, a.k, a.E, emask, ebase);
+}
+
+// More than 32 tokens: a cluster of 8 CTAs routes 32 of them.  CTA r takes an eighth of k for all
+// experts, 128 at a time: warp (p, q) has 32 of the experts and every other 32-wide block of the
+// CTA's k range.  Its router weights go from L2 straight into the registers of the warp MMAs (no
+// other warp of the CTA wants them), 20 vectors in flight per thread; the tokens' part of k is in
+// shared memory.  The two sums of a logit are added, sent to the CTA that owns the token (t % 8)
+// and added there in rank order.  Every expert's sum has the same order, so equal router rows have
+// equal logits.  Two CTAs fit an SM for up to 200 experts.
+//
+// What bounds it is the chain of latencies of one cluster (12 us), not the 6.5 MB of 509 tokens,
+// E = 128, H = 5120: 16.5 us; with 16 warps that split k in four and one CTA per SM 21.5 (the
+// GPU then holds 13 or 14 clusters at a time); by clusters of 16 as above, 32 tokens each, 30.
+constexpr int kManyTok = 32;
+constexpr int kManyCluster = 8;
+constexpr int kManySplit = 2;                        // warps that share a CTA's k
+constexpr int kManyThreads = 128 * kManySplit;
+constexpr int kManyRound = 5;                        // blocks of k a warp holds at once
+constexpr int kManyBlocks = 20;                      // 32-wide blocks of k in shared memory
+constexpr int kManyRow = kManyBlocks * 64;           // bytes of a token's row there
+constexpr int kManyOwn = kManyTok / kManyCluster;
+constexpr int kManyRed = (kManySplit - 1) * 4 * 8 * 512;
+__host__ __device__ constexpr int many_smem(int E) {
+  return kManyTok * kManyRow + kManyRed + kManyCluster * kManyOwn * E * 4;
+}
+
+__global__ void __launch_bounds__(kManyThreads, 2) k_moe_route_many(const RouteArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const uint8_t* xs = smem;
+  float4* red = reinterpret_cast<float4*>(smem + kManyTok * kManyRow);
+  // [rank][own token][expert], written by the CTAs of the cluster
+  float* recv = reinterpret_cast<float*>(smem + kManyTok * kManyRow + kManyRed);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int rp = warp / kManySplit, ks = warp % kManySplit;
+  const int rank = (int)cluster_ctarank();
+  const long long t0 = (long long)(blockIdx.x / kManyCluster) * kManyTok;
+  const int nt = (int)min((long long)kManyTok, a.T - t0);
+  const int n32 = (a.H + 31) / 32;
+  const int b0 = n32 * rank / kManyCluster, b1 = n32 * (rank + 1) / kManyCluster;
+  cluster_sync();  // every CTA of the cluster runs before its shared memory is written
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int e0 = 0; e0 < a.E; e0 += 128) {
+    float acc[2][4][4] = {};
+    const int rows = a.E - (e0 + rp * 32 + g);  // of this lane's, 8 apart
+    const __half* wp = a.wr + (e0 + rp * 32 + g) * a.ldw;
+    for (int c0 = b0; c0 < b1; c0 += kManyBlocks) {
+      const int c1 = min(b1, c0 + kManyBlocks), kend = min(a.H, c1 * 32);
+      constexpr int STEP = kManySplit * kManyRound;  // blocks of a round
+#pragma unroll 1
+      for (int r0 = 0; r0 < kManyBlocks && c0 + r0 < c1; r0 += STEP) {
+        uint4 w[kManyRound][4];
+#pragma unroll
+        for (int i = 0; i < kManyRound; ++i) {
+          const int k = (c0 + r0 + ks + kManySplit * i) * 32 + 8 * t;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            w[i][r] = make_uint4(0u, 0u, 0u, 0u);
+            if (k < kend && r * 8 < rows)
+              w[i][r] = __ldg(reinterpret_cast<const uint4*>(wp + r * 8 * a.ldw + k));
+          }
+        }
+        // the tokens' blocks, unless they are there still
+        if (r0 == 0 && (e0 == 0 || b1 - b0 > kManyBlocks)) {
+          __syncthreads();                 // everyone has read the previous ones
+          const int nv = (c1 - c0) * 4;    // vectors of a row
+          for (int i = threadIdx.x; i < kManyTok * nv; i += kManyThreads) {
+            const int m = i / nv, v = i - m * nv, k = c0 * 32 + 8 * v;
+            const bool on = m < nt && k < a.H;
+            cp_async16(smem_u32(xs + m * kManyRow + ((v ^ ((m & 1) << 2)) * 16)),
+                       on ? a.x + (t0 + m) * a.ldx + k : a.x, on);
+          }
+          cp_async_commit();
+          cp_async_wait<0>();
+          __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < kManyRound; ++i) {
+          const int j = r0 + ks + kManySplit * i;
+          if (c0 + j >= c1) break;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint4 x = *reinterpret_cast<const uint4*>(
+                xs + (n * 8 + g) * kManyRow + (((j * 4 + t) ^ ((g & 1) << 2)) * 16));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              stream_mma_16816(acc[q][n], w[i][2 * q].x, w[i][2 * q + 1].x, w[i][2 * q].y,
+                               w[i][2 * q + 1].y, x.x, x.y);
+              stream_mma_16816(acc[q][n], w[i][2 * q].z, w[i][2 * q + 1].z, w[i][2 * q].w,
+                               w[i][2 * q + 1].w, x.z, x.w);
+            }
+          }
+        }
+      }
+    }
+    if (ks > 0) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        red[(((ks - 1) * 4 + rp) * 8 + u) * 32 + lane] =
+            *reinterpret_cast<const float4*>(acc[u >> 2][u & 3]);
+    }
+    __syncthreads();
+    if (ks == 0) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        float4 v = *reinterpret_cast<const float4*>(acc[u >> 2][u & 3]);
+#pragma unroll
+        for (int s = 0; s < kManySplit - 1; ++s) {
+          const float4 o = red[((s * 4 + rp) * 8 + u) * 32 + lane];
+          v.x += o.x;
+          v.y += o.y;
+          v.z += o.z;
+          v.w += o.w;
+        }
+        const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = e0 + rp * 32 + (u >> 2) * 16 + (j >= 2 ? 8 : 0) + g;
+          const int m = (u & 3) * 8 + 2 * t + (j & 1);
+          if (e < a.E && m < nt)
+            st_dsmem_f32(mapa_shared(smem_u32(recv + (rank * kManyOwn + m / kManyCluster) * a.E + e),
+                                     m % kManyCluster), o[j]);
+        }
+      }
+    }
+    __syncthreads();  // the next experts' sums take the same place
+  }
+  cluster_sync();
+  for (int i = threadIdx.x; i < kManyOwn * a.E; i += kManyThreads) {
+    const int q = i / a.E, e = i - q * a.E;
+    if (q * kManyCluster + rank >= nt) break;
+    float v = 0.f;
+#pragma unroll
+    for (int r = 0; r < kManyCluster; ++r) v += recv[r * kManyOwn * a.E + i];
+    recv[i] = v + (a.bias ? __half2float(__ldg(a.bias + e)) : 0.f);
+  }
+  __syncthreads();
+  const int m = warp * kManyCluster + rank;
+  if (warp < kManyOwn && m < nt)
+    moe_topk(recv + warp * a.E, a.E, a.k, a.normalize != 0, a.ids + (t0 + m) * a.k,
+             a.weights + (t0 + m) * a.k);
 }
 
 // The plan of a routing the caller brings.
@@ -816,11 +956,17 @@ template <int MG>
 cudaError_t launch_route_mg(const RouteArgs& a, cudaStream_t st) {
   using C = RouteCfg<MG>;
   static BigSmem big;
-  const int grid = (a.T + C::TOK - 1) / C::TOK * kRouteCluster;
-  return launch_big(k_moe_route<MG>, big, C::SMEM, grid, 32 * C::NW, C::SMEM, st, kRouteCluster, a);
+  return launch_big(k_moe_route<MG>, big, C::SMEM, kRouteCluster, 32 * C::NW, C::SMEM, st,
+                    kRouteCluster, a);
 }
 
 cudaError_t launch_route(const RouteArgs& a, cudaStream_t st) {
+  if (a.T > RouteCfg<4>::TOK) {
+    static BigSmem big;
+    const long long grid = ((long long)a.T + kManyTok - 1) / kManyTok * kManyCluster;
+    return launch_big(k_moe_route_many, big, many_smem(kMoeMaxE), (int)grid, kManyThreads,
+                      many_smem(a.E), st, kManyCluster, a);
+  }
   return a.T <= 8 ? launch_route_mg<1>(a, st) : launch_route_mg<4>(a, st);
 }
 

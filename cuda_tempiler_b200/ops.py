@@ -28,7 +28,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    # the handle alone: building a Stream object takes 2 us, as long as a small kernel
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def workspace(dev: torch.device, nbytes: int) -> torch.Tensor | None:
@@ -242,6 +243,14 @@ def _on(dev: torch.device):
     return torch.cuda.device(dev)
 
 
+def _rows(t: torch.Tensor, name: str, dtype=torch.float16) -> int:
+    """``_check_2d``, and the row stride."""
+    st = t.stride()
+    if len(st) != 2 or st[1] != 1 or t.dtype is not dtype or not t.is_cuda:
+        _check_2d(t, name, dtype)
+    return st[0]
+
+
 def _check_same_device(dev: torch.device, **tensors) -> None:
     for name, t in tensors.items():
         if t is not None and t.device != dev:
@@ -264,7 +273,7 @@ def _check_out(out: torch.Tensor | None, M: int, N: int, dev, name: str) -> torc
     if out is None:
         return torch.empty((M, N), dtype=torch.float16, device=dev)
     _check_2d(out, name, torch.float16)
-    if tuple(out.shape) != (M, N):
+    if out.shape != (M, N):
         raise ValueError(f"{name}: expected ({M}, {N}), got {tuple(out.shape)}")
     return out
 
@@ -291,15 +300,16 @@ def _epilogue_args(N: int, M: int, bias, activation, residual):
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation {activation!r}: expected one of "
                          f"{sorted(a for a in ACTIVATIONS if a)}")
-    if bias is not None and (bias.dtype != torch.float16 or tuple(bias.shape) != (N,)
+    if bias is not None and (bias.dtype is not torch.float16 or bias.shape != (N,)
                              or bias.stride(0) != 1 and N > 1):
         raise ValueError(f"bias: expected a contiguous float16 ({N},), got {tuple(bias.shape)} "
                          f"{bias.dtype} stride {bias.stride()}")
-    if residual is not None:
-        _check_2d(residual, "residual", torch.float16)
-        if tuple(residual.shape) != (M, N):
-            raise ValueError(f"residual: expected ({M}, {N}), got {tuple(residual.shape)}")
-    return ACTIVATIONS[activation], 0 if residual is None else residual.stride(0)
+    if residual is None:
+        return ACTIVATIONS[activation], 0
+    ldr = _rows(residual, "residual")
+    if residual.shape != (M, N):
+        raise ValueError(f"residual: expected ({M}, {N}), got {tuple(residual.shape)}")
+    return ACTIVATIONS[activation], ldr
 
 
 def gemm_fp16_epilogue(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | None = None,
@@ -310,11 +320,10 @@ def gemm_fp16_epilogue(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | No
     ``out`` may be ``residual``.  Shapes and strides as ``gemm_fp16``; bias and residual 16-byte
     aligned."""
     lib = _lib.load()
-    _check_2d(A, "A", torch.float16)
-    _check_2d(B, "B", torch.float16)
+    lda, ldb = _rows(A, "A"), _rows(B, "B")
     M, K = A.shape
-    N = B.shape[0]
-    if B.shape[1] != K:
+    N, k = B.shape
+    if k != K:
         raise ValueError(f"K mismatch: A {tuple(A.shape)} B {tuple(B.shape)}")
     act, ldr = _epilogue_args(N, M, bias, activation, residual)
     dev = A.device
@@ -324,14 +333,14 @@ def gemm_fp16_epilogue(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | No
         _check_alias(out, residual, A=A, B=B, bias=bias)
     with _on(dev):
         if out is None:
-            out = torch.empty((M, N), dtype=torch.float16, device=dev)
+            out = A.new_empty((M, N))
         ws = None
         if M > STREAM_MAX_M:
             ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, 0))
         rc = lib.tempo_sm100_gemm_fp16_epilogue(
             A.data_ptr(), B.data_ptr(), out.data_ptr(), _ptr(bias), _ptr(residual), M, N, K,
-            A.stride(0), B.stride(0), out.stride(0), ldr, act, _ptr(ws),
-            0 if ws is None else ws.numel(), _stream(dev))
+            lda, ldb, out.stride(0), ldr, act, _ptr(ws), 0 if ws is None else ws.numel(),
+            _stream(dev))
     _lib.check(rc, "tempo_sm100_gemm_fp16_epilogue")
     return out
 
@@ -343,12 +352,12 @@ def _check_scales(name: str, lead: tuple, rows: int, K: int, kind: int, group: i
             raise ValueError(f"{name}: uint8 group-wise weights need scale, zero and a group_size "
                              f"that divides {K}")
         want = (*lead, K // group, rows)
-        if zero.dtype != torch.uint8 or tuple(zero.shape) != want or not zero.is_contiguous():
+        if zero.dtype is not torch.uint8 or zero.shape != want or not zero.is_contiguous():
             raise ValueError(f"{name} zero: expected a contiguous uint8 {want}, got "
                              f"{tuple(zero.shape)} {zero.dtype}")
     else:
         want = (*lead, rows)
-    if scale is None or scale.dtype != torch.float16 or tuple(scale.shape) != want \
+    if scale is None or scale.dtype is not torch.float16 or scale.shape != want \
             or not scale.is_contiguous():
         raise ValueError(f"{name} scale: expected a contiguous float16 {want}, got "
                          f"{None if scale is None else (tuple(scale.shape), scale.dtype)}")
@@ -361,14 +370,13 @@ def gemm_w8a16_epilogue(A: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
                         out: torch.Tensor | None = None) -> torch.Tensor:
     """``gemm_fp16_epilogue`` with an 8-bit weight (kinds and layouts as ``gemm_w8a16``)."""
     lib = _lib.load()
-    _check_2d(A, "A", torch.float16)
-    M, K = A.shape
-    N = W.shape[0]
     if W.dtype not in (torch.int8, torch.uint8):
         raise ValueError(f"W dtype {W.dtype}: expected int8 or uint8")
     kind = W8_INT8_PER_CHANNEL if W.dtype == torch.int8 else W8_UINT8_GROUP
-    _check_2d(W, "W", W.dtype)
-    if W.shape[1] != K:
+    lda, ldw = _rows(A, "A"), _rows(W, "W", W.dtype)
+    M, K = A.shape
+    N, k = W.shape
+    if k != K:
         raise ValueError(f"K mismatch: A {tuple(A.shape)} W {tuple(W.shape)}")
     _check_scales("W", (), N, K, kind, group_size, scale, zero)
     act, ldr = _epilogue_args(N, M, bias, activation, residual)
@@ -379,13 +387,13 @@ def gemm_w8a16_epilogue(A: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
         _check_alias(out, residual, A=A, W=W, scale=scale, zero=zero, bias=bias)
     with _on(dev):
         if out is None:
-            out = torch.empty((M, N), dtype=torch.float16, device=dev)
+            out = A.new_empty((M, N))
         ws = None
         if M > STREAM_MAX_M:
             ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, kind))
         rc = lib.tempo_sm100_gemm_w8a16_epilogue(
             A.data_ptr(), W.data_ptr(), scale.data_ptr(), _ptr(zero), out.data_ptr(), _ptr(bias),
-            _ptr(residual), M, N, K, A.stride(0), W.stride(0), out.stride(0), ldr, kind,
+            _ptr(residual), M, N, K, lda, ldw, out.stride(0), ldr, kind,
             group_size, act, _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev))
     _lib.check(rc, "tempo_sm100_gemm_w8a16_epilogue")
     return out
@@ -393,19 +401,18 @@ def gemm_w8a16_epilogue(A: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
 
 # ------------------------------------------------------------------------------ experts
 def _check_router(x, w_router, top_k, bias):
-    _check_2d(x, "x", torch.float16)
-    _check_2d(w_router, "w_router", torch.float16)
+    ldx, ldw = _rows(x, "x"), _rows(w_router, "w_router")
     E, H = w_router.shape
     if x.shape[1] != H:
         raise ValueError(f"hidden size mismatch: x {tuple(x.shape)} w_router {tuple(w_router.shape)}")
     if not 1 <= top_k <= E:
         raise ValueError(f"top_k {top_k}: expected 1 .. {E}")
-    if bias is not None and (bias.dtype != torch.float16 or tuple(bias.shape) != (E,)
+    if bias is not None and (bias.dtype is not torch.float16 or bias.shape != (E,)
                              or not bias.is_contiguous()):
         raise ValueError(f"bias: expected a contiguous float16 ({E},), got {tuple(bias.shape)} "
                          f"{bias.dtype}")
     _check_same_device(x.device, w_router=w_router, bias=bias)
-    return E, H
+    return E, H, ldx, ldw
 
 
 def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bool = True,
@@ -415,18 +422,21 @@ def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bo
     int32 and weights [T, top_k] fp32: the softmax over the chosen logits (normalize), or over all
     of them.  Any number of tokens; up to 512 experts, top_k <= 16."""
     lib = _lib.load()
-    E, H = _check_router(x, w_router, top_k, bias)
+    E, H, ldx, ldw = _check_router(x, w_router, top_k, bias)
     T, dev = x.shape[0], x.device
     with _on(dev):
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-        weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+        ids = x.new_empty((T, top_k), dtype=torch.int32)
+        weights = x.new_empty((T, top_k), dtype=torch.float32)
         if T == 0:
             return ids, weights
         rc = lib.tempo_sm100_moe_route(
             x.data_ptr(), w_router.data_ptr(), _ptr(bias), ids.data_ptr(), weights.data_ptr(), T,
-            E, H, top_k, x.stride(0), w_router.stride(0), int(normalize), _stream(dev))
+            E, H, top_k, ldx, ldw, int(normalize), _stream(dev))
     _lib.check(rc, "tempo_sm100_moe_route")
     return ids, weights
+
+
+EXPERT_KINDS = {torch.float16: 0, torch.int8: W8_INT8_PER_CHANNEL, torch.uint8: W8_UINT8_GROUP}
 
 
 def _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, group_size,
@@ -434,17 +444,16 @@ def _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, g
     _check_2d(x, "x", torch.float16)
     T, H = x.shape
     dt = w_gate_up.dtype
-    kinds = {torch.float16: 0, torch.int8: W8_INT8_PER_CHANNEL, torch.uint8: W8_UINT8_GROUP}
-    if dt not in kinds or w_down.dtype != dt:
+    kind = EXPERT_KINDS.get(dt)
+    if kind is None or w_down.dtype is not dt:
         raise ValueError(f"expert weights: float16, int8 or uint8, both alike, got {dt} and "
                          f"{w_down.dtype}")
-    kind = kinds[dt]
     if w_gate_up.dim() != 3 or w_down.dim() != 3 or not w_gate_up.is_contiguous() \
             or not w_down.is_contiguous():
         raise ValueError("expert weights: expected contiguous [E, 2I, H] and [E, H, I]")
-    E, I2, _ = w_gate_up.shape
+    E, I2, k = w_gate_up.shape
     I = I2 // 2
-    if I2 % 2 or w_gate_up.shape[2] != H or tuple(w_down.shape) != (E, H, I):
+    if I2 % 2 or k != H or w_down.shape != (E, H, I):
         raise ValueError(f"expert weights: [E, 2I, H] and [E, H, I] with H = {H}, got "
                          f"{tuple(w_gate_up.shape)} and {tuple(w_down.shape)}")
     if kind:
@@ -452,9 +461,10 @@ def _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, g
         _check_scales("down", (E,), H, I, kind, group_size, s_down, z_down)
     if gu_block < 0 or gu_block and (gu_block % 8 or I % gu_block):
         raise ValueError(f"gu_block {gu_block}: a multiple of 8 that divides {I}, or 0")
+    ldr = 0
     if residual is not None:
-        _check_2d(residual, "residual", torch.float16)
-        if tuple(residual.shape) != (T, H):
+        ldr = _rows(residual, "residual")
+        if residual.shape != (T, H):
             raise ValueError(f"residual: expected ({T}, {H}), got {tuple(residual.shape)}")
     _check_same_device(x.device, w_gate_up=w_gate_up, w_down=w_down, s_gate_up=s_gate_up,
                        z_gate_up=z_gate_up, s_down=s_down, z_down=z_down, residual=residual,
@@ -463,7 +473,7 @@ def _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, g
         _check_out(out, T, H, x.device, "out")
         _check_alias(out, residual, x=x, w_gate_up=w_gate_up, w_down=w_down, s_gate_up=s_gate_up,
                      z_gate_up=z_gate_up, s_down=s_down, z_down=z_down)
-    return T, H, E, I, kind
+    return T, H, E, I, kind, ldr
 
 
 def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor,
@@ -481,27 +491,26 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor,
     ([E, H / group_size, 2I], [E, I / group_size, H]).  ``out`` may be ``residual``.  Returns y, or
     (y, ids, weights) with return_routing."""
     lib = _lib.load()
-    T, H, E, I, kind = _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down,
-                                      group_size, gu_block, residual, out)
-    if _check_router(x, w_router, top_k, bias)[0] != E:
+    T, H, E, I, kind, ldr = _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down,
+                                           z_down, group_size, gu_block, residual, out)
+    n_routed, _, ldx, ldw = _check_router(x, w_router, top_k, bias)
+    if n_routed != E:
         raise ValueError(f"w_router names {w_router.shape[0]} experts, w_gate_up {E}")
     dev = x.device
     with _on(dev):
         if out is None:
-            out = torch.empty((T, H), dtype=torch.float16, device=dev)
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-        weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+            out = x.new_empty((T, H))
+        ids = x.new_empty((T, top_k), dtype=torch.int32)
+        weights = x.new_empty((T, top_k), dtype=torch.float32)
         if T:
             # a call's own workspace: nothing in it outlives the call or has to be cleared
-            ws = torch.empty(lib.tempo_sm100_moe_workspace_bytes(T, top_k, I), dtype=torch.uint8,
-                             device=dev)
+            ws = x.new_empty(lib.tempo_sm100_moe_workspace_bytes(T, top_k, I), dtype=torch.uint8)
             rc = lib.tempo_sm100_moe_layer(
                 x.data_ptr(), w_router.data_ptr(), _ptr(bias), w_gate_up.data_ptr(),
                 w_down.data_ptr(), _ptr(s_gate_up), _ptr(z_gate_up), _ptr(s_down), _ptr(z_down),
                 _ptr(residual), out.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, E, H, I,
-                top_k, x.stride(0), w_router.stride(0),
-                0 if residual is None else residual.stride(0), out.stride(0), kind, group_size,
-                gu_block, int(normalize), ws.data_ptr(), ws.numel(), _stream(dev))
+                top_k, ldx, ldw, ldr, out.stride(0), kind, group_size, gu_block, int(normalize),
+                ws.data_ptr(), ws.numel(), _stream(dev))
             _lib.check(rc, "tempo_sm100_moe_layer")
     return (out, ids, weights) if return_routing else out
 
@@ -516,8 +525,8 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     [T, k] fp32.  An id outside [0, E) names no expert (a token with none gets its residual, or
     zero); an expert a token names twice counts with the sum of the two weights."""
     lib = _lib.load()
-    T, H, E, I, kind = _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down,
-                                      group_size, gu_block, residual, out)
+    T, H, E, I, kind, ldr = _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down,
+                                           z_down, group_size, gu_block, residual, out)
     dev = x.device
     if ids.dtype != torch.int32 or ids.dim() != 2 or ids.shape[0] != T or ids.shape[1] < 1 \
             or not ids.is_contiguous():
@@ -531,15 +540,13 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     top_k = ids.shape[1]
     with _on(dev):
         if out is None:
-            out = torch.empty((T, H), dtype=torch.float16, device=dev)
+            out = x.new_empty((T, H))
         if T:
-            ws = torch.empty(lib.tempo_sm100_moe_workspace_bytes(T, top_k, I), dtype=torch.uint8,
-                             device=dev)
+            ws = x.new_empty(lib.tempo_sm100_moe_workspace_bytes(T, top_k, I), dtype=torch.uint8)
             rc = lib.tempo_sm100_moe_experts(
                 x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(),
                 w_down.data_ptr(), _ptr(s_gate_up), _ptr(z_gate_up), _ptr(s_down), _ptr(z_down),
-                _ptr(residual), out.data_ptr(), T, E, H, I, top_k, x.stride(0),
-                0 if residual is None else residual.stride(0), out.stride(0), kind, group_size,
-                gu_block, ws.data_ptr(), ws.numel(), _stream(dev))
+                _ptr(residual), out.data_ptr(), T, E, H, I, top_k, x.stride(0), ldr,
+                out.stride(0), kind, group_size, gu_block, ws.data_ptr(), ws.numel(), _stream(dev))
             _lib.check(rc, "tempo_sm100_moe_experts")
     return out
