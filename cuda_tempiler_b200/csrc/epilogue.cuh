@@ -1,7 +1,7 @@
 // The GEMM with a fused epilogue, y = act(A W^T + bias) + residual: which kernel runs.
 //
 //   M <= 16    k_stream_linear (stream.cuh)
-//   M <= 384   k_epi_swap (swap_tile.cuh); 8-bit weights up to 1279 rows
+//   M <= 512   k_epi_swap (swap_tile.cuh); 8-bit weights up to 1279 rows
 //   above      the 2-CTA tiles the shipped dispatcher plans for the fp16 problem, with the epilogue
 //              on the accumulator; 8-bit weights are expanded to fp16 first, the per-channel kind
 //              without its scale, which multiplies the fp32 accumulator instead (an int8 value is

@@ -26,8 +26,9 @@
 // transposed; bias, activation and residual then work on 8 consecutive columns per thread with
 // 16-byte accesses, the residual of the next rows in flight meanwhile.
 //
-// Warps: 0 TMA, 1 MMA (and TMEM), 2-5 epilogue; 8-bit weights: 6 TMA of the raw tiles, 7-14
-// unpacking.
+// Warps: 0 TMA, 1 MMA (and TMEM), two groups of four for the epilogue that take its chunks of 16
+// rows in turn (256 x 18944 x 3840: 38.6 us with one group, 35.8 with two); 8-bit weights: one warp
+// for TMA of the raw tiles, eight for unpacking.
 #pragma once
 
 namespace tempo_sm100 {
@@ -45,10 +46,19 @@ __device__ __forceinline__ bool named_barrier_and(int id, int threads, bool p) {
   return r != 0;
 }
 
+// True in one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 constexpr int kSwapMaxRows = 384;  // of a tile: two accumulators of 192 columns
 constexpr int kSwapRawBytes = 128 * 64 + 1024;           // raw tile, scale row, zero row
 constexpr int kSwapStageRow = 132;                       // floats of a transposed output row
-constexpr int kSwapEpiBytes = 16 * kSwapStageRow * 4 + 512;
+constexpr int kSwapStageBytes = 16 * kSwapStageRow * 4;  // one group's
 constexpr int kSwapBarBytes = 512;
 constexpr int kSwapMaxSlots = 8;
 
@@ -60,6 +70,7 @@ struct SwapArgs {
   int nx, nr;                 // operand slots, raw tiles
   int x_bytes;                // one operand slot: 16 KB of weights, the activations
   int bufs;                   // accumulator buffers (2 when they fit 512 columns)
+  int epis;                   // groups of epilogue warps at work
   int unit;                   // shares are multiples of it (k-blocks)
   __half* C;
   long long ldc;
@@ -117,7 +128,8 @@ struct EpiCols {
   }
   __device__ __forceinline__ uint4 apply(const EpiArgs& e, float (&o)[8], uint4 res) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = epi_act(fmaf(o[j], scale[j], bias[j]), e.act);
+    for (int j = 0; j < 8; ++j) o[j] = fmaf(o[j], scale[j], bias[j]);
+    epi_act(o, e.act);
     if (e.res) {
       float r[8];
       unpack_half8(res, r);
@@ -134,7 +146,7 @@ struct EpiCols {
 };
 
 template <int WQ>
-constexpr int kSwapThreads = WQ ? 15 * 32 : 6 * 32;
+constexpr int kSwapThreads = WQ ? 19 * 32 : 10 * 32;
 
 // LG: groups of unpacking warps.  2: four warps fill a slot, the others the next one (a slot's turn,
 // its data, the fence and the arrival take a warp longer than a k-block of 8-bit weights may); a
@@ -149,8 +161,9 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint8_t* raw = smem + a.nx * a.x_bytes;
-  float* stage = reinterpret_cast<float*>(raw + a.nr * kSwapRawBytes);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(stage) + kSwapEpiBytes);
+  float* stage0 = reinterpret_cast<float*>(raw + a.nr * kSwapRawBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(stage0) +
+                                               a.epis * kSwapStageBytes);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * kSwapMaxSlots + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t bar0 = smem_u32(bars);
@@ -175,7 +188,7 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull(b), 1);
-      mbar_init(tempty(b), 4);
+      mbar_init(tempty(b), 4 * a.epis);
     }
     mbar_init(done_bar, 1);
     *abort_flag = 0;
@@ -234,7 +247,7 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
       for (int j = it > a.nx ? it - a.nx : 0; j < it; ++j)
         mbar_drain(xfull(j % a.nx), (uint32_t)((j / a.nx) & 1), 100000000ull);
     }
-  } else if (WQ && warp == 6) {
+  } else if (WQ && warp == 10) {
     // ------------------------------------------------------------------ TMA: raw weights
     if (lane == 0) {
       const uint64_t pol_w = policy_evict_first(), pol = policy_evict_last();
@@ -274,7 +287,6 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
     const uint32_t hi = (uint32_t)(sdesc_k_sw128(0) >> 32);
     auto low = [](uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | (1u << 16); };
     auto desc = [&](uint32_t lo) { return (uint64_t)hi << 32 | lo; };
-    const bool one = lane == 0;
     int lu = 0, s = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -292,7 +304,7 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
         tc_fence_after();
         const uint32_t wa = low(x0 + s * a.x_bytes);
         const uint32_t ba = wa + (16384 >> 4), bb = ba + a.n * 8;  // second group: n rows further
-        if (one) {
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_f16_ss(d, desc(wa + 2 * k), desc(ba + 2 * k), idesc, k ? 1u : add);
@@ -311,19 +323,21 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
         }
       }
       if (!ok) break;
-      if (one) umma_commit(tfull(buf));
+      if (elect_one()) umma_commit(tfull(buf));
       __syncwarp();
     }
-    if (one) {
+    if (elect_one()) {
       umma_commit(done_bar);
       mbar_drain(done_bar, 0, 100000000ull);
     }
     __syncwarp();
-  } else if (warp < 6) {
+  } else if (warp < 2 + 4 * a.epis) {
     // ------------------------------------------------------------------ epilogue
     const int quad = warp & 3, row = quad * 32 + lane;  // TMEM lane = weight row of the tile
     const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16);
-    const int tid = threadIdx.x - 64;
+    const int grp = (warp - 2) >> 2;                    // takes the chunks grp, grp + epis, ...
+    const int tid = (threadIdx.x - 64) & 127, bar = 1 + grp;
+    float* stage = stage0 + grp * (kSwapStageBytes / 4);
     const int v8 = (tid & 15) * 8, trow = tid >> 4;     // columns and first output row of a chunk
     int lu = 0;
     for (; segs.next(sg); ++lu) {
@@ -346,21 +360,22 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
       EpiCols ec;
       if (whole) {
         ec.load(a.epi, WQ == kWInt8PerChannel ? a.scale : nullptr, n0, n_ok);
-        if (a.epi.res) load_res(0);
+        if (a.epi.res) load_res(grp);
       }
       // one warp's wait may run out where another's did not: all four go on or none does
-      if (!named_barrier_and(1, 128, mbar_wait(tfull(buf), (uint32_t)((lu / a.bufs) & 1),
-                                               abort_flag, 36)))
+      if (!named_barrier_and(bar, 128, mbar_wait(tfull(buf), (uint32_t)((lu / a.bufs) & 1),
+                                                 abort_flag, 36)))
         break;
       tc_fence_after();
       // a partial tile: part 0 of this CTA when the tile began in an earlier share, else part 1
       float* dst = a.part + (blockIdx.x * 2LL + (sg.kb0 > 0 ? 0 : 1)) * a.rows * 128 + row;
+      if (grp >= chunks && lane == 0) mbar_arrive(tempty(buf));
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
+      for (int c = grp; c < chunks; c += a.epis) {
         uint32_t v[16];
         tmem_ld_x16(t_acc + c * 16, v);
         tmem_wait_ld();
-        if (c == chunks - 1) {
+        if (c + a.epis >= chunks) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(tempty(buf));
@@ -370,12 +385,12 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
           for (int j = 0; j < 16; ++j) __stcg(dst + (c * 16 + j) * 128, __uint_as_float(v[j]));
           continue;
         }
-        named_barrier_sync(1, 128);  // the previous chunk has been read
+        named_barrier_sync(bar, 128);  // the previous chunk has been read
 #pragma unroll
         for (int j = 0; j < 16; ++j) stage[j * kSwapStageRow + row] = __uint_as_float(v[j]);
-        named_barrier_sync(1, 128);
+        named_barrier_sync(bar, 128);
         const uint4 cur[2] = {res[0], res[1]};
-        if (a.epi.res && c + 1 < chunks) load_res(c + 1);
+        if (a.epi.res && c + a.epis < chunks) load_res(c + a.epis);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int m = c * 16 + trow + 8 * i;
@@ -389,14 +404,14 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
         }
       }
     }
-  } else if (WQ) {
+  } else if (WQ && warp > 10) {
     // ------------------------------------------------------------------ unpacking
     // Group g takes the k-blocks g, g + LG, ...; warp d of it fills rows R d .. R d + R - 1 of the
     // slot, 4 lanes per row: 16 weights of lane (row, lc) are the fp16 granules 2 lc, 2 lc + 1, and
     // granule j of row r lives at j ^ (r % 8) (the operand's 128-byte swizzle); neither reads nor
     // stores conflict.
     constexpr int R = 16 * LG, L = R / 8;  // rows per warp, chunks per lane
-    const int grp = LG == 2 ? (warp - 7) >> 2 : 0, d = LG == 2 ? (warp - 7) & 3 : warp - 7;
+    const int grp = LG == 2 ? (warp - 11) >> 2 : 0, d = LG == 2 ? (warp - 11) & 3 : warp - 11;
     const int lr = lane >> 2, lc = lane & 3;
     int s = grp, r = grp;
     uint32_t ph = 1, rph = 0;
@@ -458,36 +473,49 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
 // The tiles that k_epi_swap's shares cut: their parts added in k order, then the epilogue.  One CTA
 // per tile and 16 output rows, 8 columns of a row per thread.
 template <int WQ>
-__global__ void __launch_bounds__(256) k_swap_finish(const SwapArgs a, int ctas) {
-  pdl_wait();
-  pdl_launch_dependents();
+__global__ void __launch_bounds__(256, 3) k_swap_finish(const SwapArgs a, int ctas) {
   const int tile = blockIdx.x;
   const SwapShare share(a.tiles * a.num_kb, ctas, a.unit);
   const int first = share.owner(tile * a.num_kb), last = share.owner((tile + 1) * a.num_kb - 1);
   const int v8 = (threadIdx.x & 15) * 8, r = blockIdx.y * 16 + (threadIdx.x >> 4);
   const int wt = tile / a.mt, m = (tile - wt * a.mt) * a.rows + r;
   const int n0 = wt * 128 + v8;
-  if (first == last || m >= a.M || n0 >= a.N) return;
+  const bool on = first != last && m < a.M && n0 < a.N;
+  // What k_epi_swap does not write can be read while it still runs: it started this launch only
+  // after its own wait for whatever wrote these.
   uint4 res = make_uint4(0u, 0u, 0u, 0u);
-  if (a.epi.res)
+  if (on && a.epi.res)
     res = *reinterpret_cast<const uint4*>(a.epi.res + (long long)m * a.epi.ldr + n0);
   EpiCols ec;
-  ec.load(a.epi, WQ == kWInt8PerChannel ? a.scale : nullptr, n0, true);
+  ec.load(a.epi, WQ == kWInt8PerChannel ? a.scale : nullptr, n0, on);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!on) return;
   float o[8] = {};
-#pragma unroll 4
-  for (int c = first; c <= last; ++c) {
-    const int part = share.begin(c) > tile * a.num_kb ? 0 : 1;
-    const float4* src = reinterpret_cast<const float4*>(
-        a.part + ((c * 2LL + part) * a.rows + r) * 128 + v8);
-    const float4 lo = __ldcg(src), hi = __ldcg(src + 1);
-    o[0] += lo.x;
-    o[1] += lo.y;
-    o[2] += lo.z;
-    o[3] += lo.w;
-    o[4] += hi.x;
-    o[5] += hi.y;
-    o[6] += hi.z;
-    o[7] += hi.w;
+  for (int c0 = first; c0 <= last; c0 += 4) {
+    float4 lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + i;
+      lo[i] = hi[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c > last) continue;
+      const int part = share.begin(c) > tile * a.num_kb ? 0 : 1;
+      const float4* src = reinterpret_cast<const float4*>(
+          a.part + ((c * 2LL + part) * a.rows + r) * 128 + v8);
+      lo[i] = __ldcg(src);
+      hi[i] = __ldcg(src + 1);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[0] += lo[i].x;
+      o[1] += lo[i].y;
+      o[2] += lo[i].z;
+      o[3] += lo[i].w;
+      o[4] += hi[i].x;
+      o[5] += hi[i].y;
+      o[6] += hi[i].z;
+      o[7] += hi[i].w;
+    }
   }
   *reinterpret_cast<uint4*>(a.C + (long long)m * a.ldc + n0) = ec.apply(a.epi, o, res);
 }
@@ -495,7 +523,7 @@ __global__ void __launch_bounds__(256) k_swap_finish(const SwapArgs a, int ctas)
 namespace {
 
 struct SwapPlan {
-  int n, groups, rows, mt, x_bytes, nx, nr, bufs, tiles, num_kb, ctas, unit, smem;
+  int n, groups, rows, mt, x_bytes, nx, nr, bufs, epis, tiles, num_kb, ctas, unit, smem;
   size_t ws_bytes;  // 0: whole tiles, no workspace
 };
 
@@ -513,15 +541,21 @@ double epi_swap_cost(SwapPlan& p, int wkind, int M, int N, int K, int sms, size_
   p.num_kb = (K + 63) / 64;
   p.bufs = p.rows <= 256 ? 2 : 1;
   p.x_bytes = 16384 + p.rows * 128;
-  const int room = kMaxDynSmem - 1024 - kSwapEpiBytes - kSwapBarBytes;
-  p.nx = std::min(room / p.x_bytes, kSwapMaxSlots);
-  p.nr = 0;
-  if (wkind) {
-    // up to 4 operand slots that leave at least 4 raw tiles
-    p.nx = std::max(2, std::min(4, (room - 4 * kSwapRawBytes) / p.x_bytes));
-    p.nr = std::min((room - p.nx * p.x_bytes) / kSwapRawBytes, kSwapMaxSlots) & ~1;
+  // One group of epilogue warps where the staging of the second would cost an operand slot: 8-bit
+  // weights above 320 rows, which then have 2 (333 x 5120 x 17408: 69 us against 65).
+  const int room = kMaxDynSmem - 1024 - kSwapBarBytes;
+  for (p.epis = 2;; --p.epis) {
+    const int left = room - p.epis * kSwapStageBytes;
+    p.nx = std::min(left / p.x_bytes, kSwapMaxSlots);
+    p.nr = 0;
+    if (wkind) {
+      // up to 4 operand slots that leave at least 4 raw tiles
+      p.nx = std::max(2, std::min(4, (left - 4 * kSwapRawBytes) / p.x_bytes));
+      p.nr = std::min((left - p.nx * p.x_bytes) / kSwapRawBytes, kSwapMaxSlots) & ~1;
+    }
+    if (p.epis == 1 || p.nx > 2) break;
   }
-  p.smem = 1024 + p.nx * p.x_bytes + p.nr * kSwapRawBytes + kSwapEpiBytes + kSwapBarBytes;
+  p.smem = 1024 + p.nx * p.x_bytes + p.nr * kSwapRawBytes + p.epis * kSwapStageBytes + kSwapBarBytes;
   const double wb = 128.0 * 64 * (wkind == 0 ? 2 : 1) / p.mt;
   auto kb_cycles = [&](int active) {
     return std::max({p.groups * 4.0 * std::max(45.0, p.n / 2.0), p.rows * 128.0 / 64.0, wb / 30.0,
@@ -596,6 +630,7 @@ cudaError_t launch_epi_swap(const Problem& pr, cudaStream_t st) {
   a.nr = p.nr;
   a.x_bytes = p.x_bytes;
   a.bufs = p.bufs;
+  a.epis = p.epis;
   a.unit = p.unit;
   a.C = static_cast<__half*>(pr.C);
   a.ldc = pr.ldc;
