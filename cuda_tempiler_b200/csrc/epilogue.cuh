@@ -1,7 +1,7 @@
 // The GEMM with a fused epilogue, y = act(A W^T + bias) + residual: which kernel runs.
 //
-//   M <= 16    k_stream_linear (stream.cuh)
-//   M <= 512   k_epi_swap (swap_tile.cuh); 8-bit weights up to 1279 rows
+//   M <= 16    k_stream_linear (stream.cuh) where a CTA's weight rows are few (stream_epilogue)
+//   M <= 384   k_epi_swap (swap_tile.cuh); 8-bit weights up to 1279 rows
 //   above      the 2-CTA tiles the shipped dispatcher plans for the fp16 problem, with the epilogue
 //              on the accumulator; 8-bit weights are expanded to fp16 first, the per-channel kind
 //              without its scale, which multiplies the fp32 accumulator instead (an int8 value is
@@ -33,13 +33,42 @@ __global__ void __launch_bounds__(256)
 
 namespace {
 
-// Above kStreamMaxM rows: the swapped tiles, or the 2-CTA ones (8-bit weights expanded first).
-// Measured, swapped / 2-CTA us: fp16 400 x 3840 x 4096 31 / 36, 512 x 8192 x 3840 61 / 41,
-// 1024 x 15360 x 3840 186 / 106; 8-bit 512 x 10240 x 5120 91 / 93, 1024 x 5120 x 8192 97 / 118,
-// 1536 x 5120 x 17408 304 / 265, 4096 x 15360 x 3840 560 / 361.
+// Up to kStreamMaxM rows: the stream while a CTA's share of the weight rows fits a piece or two
+// (every further piece reads the activations again and adds up its warps' sums), above that the
+// swapped tiles.  Measured, stream / swapped us at 8 and at 16 rows (N x K):
+//   fp16   3840 x 4096   8.5 / 11.1   9.2 / 11.3     5120 x 8192  18.1 / 18.5  21.5 / 18.7
+//          8192 x 3840  17.4 / 15.2  22.1 / 15.3    15360 x 3840  26.7 / 21.4  33.1 / 21.2
+//   int8   5120 x 8192  13.5 / 17.5  15.1 / 18.5     8192 x 3840  14.7 / 14.9  17.6 / 15.6
+//         10240 x 5120  18.6 / 19.6  21.1 / 20.2    15360 x 3840  22.3 / 20.0  25.9 / 20.3
+// Group-wise weights always (5120 x 8192 14.3 / 20.9 and 18.0 / 21.7, 15360 x 3840 23.6 / 25.9 and
+// 30.3 / 25.9): the stream takes them as they are, the tiles round each to fp16.
+bool stream_epilogue(int M, int N, int wkind) {
+  if (M > kStreamMaxM) return false;
+  const int sms = current_sms() > 0 ? current_sms() : 1;
+  const int rows = (N + sms - 1) / sms;
+  switch (wkind) {
+    case kWFp16: return rows <= (M <= 8 ? 48 : 32);
+    case kWInt8PerChannel: return rows <= (M <= 8 ? 96 : 48);
+    default: return true;
+  }
+}
+
+// Above them: the swapped tiles, or the 2-CTA ones (8-bit weights expanded first).  Measured,
+// swapped / 2-CTA us: fp16 15360 x 3840 at 384 rows 50 / 56 (385 rows), 5120 x 17408 72 / 96,
+// 3840 x 4096 29 / 30; from 385 rows on a second tile of rows would be mostly padding.  8-bit
+// 1024 x 5120 x 8192 97 / 118, 15360 x 3840 at 1280 rows 172 / 154, 1536 x 5120 x 17408 304 / 265.
 bool swap_epilogue(int M, int N, int K, int wkind, size_t ws_bytes) {
   if (wkind == kWFp16) return M <= kSwapMaxRows;
   return M < 1280 || ws_bytes < kExpandOffset + expand_ws_bytes(N, K);
+}
+
+// Workspace the kernel of choice would like (0: none).
+size_t epilogue_ws_bytes(int M, int N, int K, int wkind) {
+  if (stream_epilogue(M, N, wkind)) return 0;
+  if (swap_epilogue(M, N, K, wkind, ~(size_t)0))
+    return epi_swap_plan(wkind, M, N, K, std::max(1, current_sms()), ~(size_t)0).ws_bytes;
+  const size_t ws = tempo_sm100_workspace_bytes(M, N, K, 0);
+  return wkind == kWFp16 ? ws : std::max(ws, (size_t)kExpandOffset) + expand_ws_bytes(N, K);
 }
 
 cudaError_t run_pair_epi(const Problem& pr, const Hyper& h, cudaStream_t st) {
@@ -54,20 +83,22 @@ cudaError_t run_pair_epi(const Problem& pr, const Hyper& h, cudaStream_t st) {
 }
 
 cudaError_t run_epilogue(const Problem& pr, cudaStream_t st) {
-  if (pr.M <= kStreamMaxM)
+  const size_t cap = pr.ws ? pr.ws_bytes : 0;
+  // the stream needs no workspace; without one the swapped tiles would run whole, on few SMs
+  if (stream_epilogue(pr.M, pr.N, pr.wkind) ||
+      (pr.M <= kStreamMaxM && cap < epilogue_ws_bytes(pr.M, pr.N, pr.K, pr.wkind)))
     return run_stream({static_cast<const __half*>(pr.A), static_cast<const uint8_t*>(pr.W),
                        static_cast<const __half*>(pr.scale), static_cast<const uint8_t*>(pr.zero),
                        static_cast<__half*>(pr.C), pr.epi, pr.M, pr.N, pr.K, pr.lda, pr.ldw,
                        pr.ldc, pr.group > 0 ? pr.group : 1},
                       pr.wkind, st);
-  if (swap_epilogue(pr.M, pr.N, pr.K, pr.wkind, pr.ws ? pr.ws_bytes : 0)) {
+  if (swap_epilogue(pr.M, pr.N, pr.K, pr.wkind, cap)) {
     switch (pr.wkind) {
       case kWFp16: return launch_epi_swap<kWFp16>(pr, st);
       case kWInt8PerChannel: return launch_epi_swap<kWInt8PerChannel>(pr, st);
       default: return launch_epi_swap<kWUint8Group>(pr, st);
     }
   }
-  const size_t cap = pr.ws ? pr.ws_bytes : 0;
   tempo::gen::Choice c{};
   tempo::gen::GemmParams p{};
   p.M = pr.M; p.N = pr.N; p.K = pr.K;
@@ -102,15 +133,6 @@ cudaError_t run_epilogue(const Problem& pr, cudaStream_t st) {
     return run_pair_epi(q, h, st);
   }
   return run_pair_epi(pr, h, st);
-}
-
-// Workspace run_epilogue would like (0: none).
-size_t epilogue_ws_bytes(int M, int N, int K, int wkind) {
-  if (M <= kStreamMaxM) return 0;
-  if (swap_epilogue(M, N, K, wkind, ~(size_t)0))
-    return epi_swap_plan(wkind, M, N, K, std::max(1, current_sms()), ~(size_t)0).ws_bytes;
-  const size_t ws = tempo_sm100_workspace_bytes(M, N, K, 0);
-  return wkind == kWFp16 ? ws : std::max(ws, (size_t)kExpandOffset) + expand_ws_bytes(N, K);
 }
 
 }  // namespace

@@ -532,7 +532,7 @@ struct SwapPlan {
 // 64 B/cycle, its weights from HBM at 30 B/cycle of an SM and at 3400 of the GPU.
 double epi_swap_cost(SwapPlan& p, int wkind, int M, int N, int K, int sms, size_t ws_bytes,
                      int mt) {
-  const int want = (M + mt - 1) / mt;
+  const int want = (int)(((long long)M + mt - 1) / mt);
   p.groups = want > 256 ? 2 : 1;
   p.n = ((want + p.groups - 1) / p.groups + 15) / 16 * 16;
   p.rows = p.groups * p.n;
@@ -566,8 +566,8 @@ double epi_swap_cost(SwapPlan& p, int wkind, int M, int N, int K, int sms, size_
   const int waves = (p.tiles + sms - 1) / sms;
   const double whole = (double)waves * p.num_kb * kb_cycles(std::min(p.tiles, sms)) + tail;
   // equal shares of at least 4 k-blocks; the partial tiles' way through L2 and one more launch
-  const int total = p.tiles * p.num_kb;
-  const int ctas = std::min(sms, std::max(1, total / 4));
+  const long long total = (long long)p.tiles * p.num_kb;
+  const int ctas = (int)std::min<long long>(sms, std::max(1LL, total / 4));
   const double share =
       (double)((total + ctas - 1) / ctas) * kb_cycles(ctas) + 5000.0 + 10.0 * p.rows + tail;
   const size_t need = kCounterBytes + 2 * (size_t)ctas * p.rows * 128 * sizeof(float);

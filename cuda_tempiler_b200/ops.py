@@ -19,8 +19,8 @@ from ._lib import NotCovered, W8_INT8_PER_CHANNEL, W8_UINT8_GROUP  # noqa: F401
 _ws_cache: dict = {}
 # the W8A16 prefill's fp16 weight copy starts after the workspace's 64 KiB counter prefix
 EXPAND_OFFSET = 65536
-# rows up to which a product with an epilogue streams its weights (no workspace)
-STREAM_MAX_M = 16
+# a product with an epilogue of at most so many rows and columns streams its weights: no workspace
+STREAM_MAX_M, STREAM_MAX_N = 16, 4096
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -29,7 +29,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _stream(dev: torch.device) -> int:
     # the handle alone: building a Stream object takes 2 us, as long as a small kernel
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if dev.index is None else dev.index)
 
 
 def workspace(dev: torch.device, nbytes: int) -> torch.Tensor | None:
@@ -335,7 +336,7 @@ def gemm_fp16_epilogue(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | No
         if out is None:
             out = A.new_empty((M, N))
         ws = None
-        if M > STREAM_MAX_M:
+        if M > STREAM_MAX_M or N > STREAM_MAX_N:
             ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, 0))
         rc = lib.tempo_sm100_gemm_fp16_epilogue(
             A.data_ptr(), B.data_ptr(), out.data_ptr(), _ptr(bias), _ptr(residual), M, N, K,
@@ -389,7 +390,7 @@ def gemm_w8a16_epilogue(A: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
         if out is None:
             out = A.new_empty((M, N))
         ws = None
-        if M > STREAM_MAX_M:
+        if M > STREAM_MAX_M or N > STREAM_MAX_N:
             ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, kind))
         rc = lib.tempo_sm100_gemm_w8a16_epilogue(
             A.data_ptr(), W.data_ptr(), scale.data_ptr(), _ptr(zero), out.data_ptr(), _ptr(bias),

@@ -129,6 +129,67 @@ def test_long_shares(dev, kind, group, M, N, K):
         assert torch.equal(y, call(A, w, group, residual=res))
 
 
+@pytest.mark.parametrize("kind,group", [("fp16", 0), ("int8", 0), ("uint8", 128)])
+@pytest.mark.parametrize("M,N", [(1, 7168), (5, 15360), (8, 8192), (9, 5120), (16, 7680), (16, 20480)])
+def test_few_rows_many_columns(dev, kind, group, M, N):
+    """Up to 16 rows on both sides of the choice between the stream and the tiles, and the answer
+    without a workspace."""
+    from cuda_tempiler_b200 import _lib
+    K = 1152
+    A, w = rand(M, K, seed=M), weights(kind, N, K, group, seed=5)
+    bias, res = rand(N, seed=7), rand(M, N, seed=6)
+    check(call(A, w, group, bias=bias, activation="gelu_tanh", residual=res), A, w, group, bias,
+          "gelu_tanh", res)
+    out, lib = poison(M, N), _lib.load()
+    st = torch.cuda.current_stream().cuda_stream
+    tail = (out.data_ptr(), bias.data_ptr(), res.data_ptr(), M, N, K, K, K, N, N)
+    act = 4  # TEMPO_ACT_GELU_TANH
+    if kind == "fp16":
+        rc = lib.tempo_sm100_gemm_fp16_epilogue(A.data_ptr(), w[0].data_ptr(), *tail, act, None, 0,
+                                                st)
+    else:
+        rc = lib.tempo_sm100_gemm_w8a16_epilogue(
+            A.data_ptr(), w[0].data_ptr(), w[1].data_ptr(),
+            None if w[2] is None else w[2].data_ptr(), *tail, 1 if kind == "int8" else 2, group,
+            act, None, 0, st)
+    assert rc == 0
+    check(out, A, w, group, bias, "gelu_tanh", res)
+
+
+@pytest.mark.parametrize("kind,group", [("fp16", 0), ("int8", 0), ("uint8", 128)])
+@pytest.mark.parametrize("M,N,K", [(40, 528, 4096), (300, 272, 2048), (700, 400, 1152)])
+def test_without_a_workspace(dev, kind, group, M, N, K):
+    """The tiles run whole; 8-bit weights are not expanded."""
+    from cuda_tempiler_b200 import _lib
+    A, w = rand(M, K, seed=M), weights(kind, N, K, group, seed=5)
+    res = rand(M, N, seed=6)
+    out, lib = poison(M, N), _lib.load()
+    st = torch.cuda.current_stream().cuda_stream
+    tail = (out.data_ptr(), None, res.data_ptr(), M, N, K, K, K, N, N)
+    if kind == "fp16":
+        rc = lib.tempo_sm100_gemm_fp16_epilogue(A.data_ptr(), w[0].data_ptr(), *tail, 0, None, 0, st)
+    else:
+        rc = lib.tempo_sm100_gemm_w8a16_epilogue(
+            A.data_ptr(), w[0].data_ptr(), w[1].data_ptr(),
+            None if w[2] is None else w[2].data_ptr(), *tail, 1 if kind == "int8" else 2, group, 0,
+            None, 0, st)
+    assert rc == 0
+    check(out, A, w, group, None, "none", res)
+
+
+@pytest.mark.parametrize("M", [40, 300])
+def test_infinite_rows_stay_apart_in_tiles(dev, M):
+    """As above for the tiles, whose MMA has the rows as its N side; k is cut into shares."""
+    N, K = 264, 4096
+    A, w = rand(M, K, seed=8), weights("fp16", N, K, 0)
+    clean = call(A, w, 0)
+    A[1, 3], A[M - 1, K - 1] = float("inf"), float("nan")
+    y = call(A, w, 0)
+    rest = [m for m in range(M) if m not in (1, M - 1)]
+    assert torch.equal(y[rest], clean[rest])
+    assert torch.isnan(y[M - 1]).all() and not torch.isfinite(y[1]).any()
+
+
 @pytest.mark.parametrize("kind,group", [("fp16", 0), ("int8", 0), ("uint8", 64)])
 @pytest.mark.parametrize("M", [1, 7, 16])
 def test_infinite_rows_stay_apart(dev, kind, group, M):
