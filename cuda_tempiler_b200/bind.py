@@ -126,14 +126,20 @@ def _stock_epilogue(y, activation, residual):
     return y if residual is None else y + residual
 
 
-def _fused(x2, N, bias, activation, residual, run):
-    """run(residual rows) where the epilogue kernels cover the extra operands, else None."""
-    res = None if residual is None else residual.reshape(-1, N)
-    if res is not None and (res.dtype != torch.float16 or res.device != x2.device
-                            or res.shape[0] != x2.shape[0] or res.stride(1) != 1
-                            or res.stride(0) % 8 or not _aligned(res)):
+def _fused(x, weight, bias, activation, residual, run):
+    """run(residual rows) where the epilogue kernels cover the extra operands, else None.  They
+    have no backward pass: with gradients to record the stock operators run."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, weight, bias, residual)):
         return None
-    if bias is not None and (bias.dtype != torch.float16 or bias.device != x2.device
+    N = weight.shape[0]
+    if residual is not None and residual.shape != (*x.shape[:-1], N):
+        return None
+    res = None if residual is None else residual.reshape(-1, N)
+    if res is not None and (res.dtype != torch.float16 or res.device != x.device
+                            or res.stride(1) != 1 or res.stride(0) % 8 or not _aligned(res)):
+        return None
+    if bias is not None and (bias.dtype != torch.float16 or bias.device != x.device
                              or not bias.is_contiguous() or not _aligned(bias)):
         return None
     try:
@@ -154,8 +160,8 @@ def linear_fp16(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
         if covered_fp16(x2, weight):
             N = weight.shape[0]
             if fuse:
-                y = _fused(x2, N, bias, activation, residual, lambda res: ops.gemm_fp16_epilogue(
-                    x2, weight, bias, activation, res))
+                y = _fused(x, weight, bias, activation, residual,
+                           lambda res: ops.gemm_fp16_epilogue(x2, weight, bias, activation, res))
                 if y is not None:
                     _count("tempo")
                     return y.reshape(*x.shape[:-1], N)
@@ -193,7 +199,7 @@ def linear_w8a16(x: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
         if covered_w8a16(x2, W, scale, zero, group_size):
             N = W.shape[0]
             if fuse:
-                y = _fused(x2, N, bias, activation, residual, lambda res: ops.gemm_w8a16_epilogue(
+                y = _fused(x, W, bias, activation, residual, lambda res: ops.gemm_w8a16_epilogue(
                     x2, W, scale, zero, group_size, bias, activation, res))
                 if y is not None:
                     _count("tempo")

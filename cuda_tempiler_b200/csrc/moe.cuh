@@ -6,8 +6,8 @@
 //   k_moe_down     y[t][n] = res[t][n] + sum_e sum_i down_e[n][i] h[(t, e)][i]
 //
 // The bytes are the weights of the reached experts, read once each whatever the number of
-// tokens; everything else is small.  The products are those of stream.cuh: weights straight from
-// HBM into the registers of warp MMAs, fp32 sums, 8-bit weights as exact integers.
+// tokens; everything else is small.  The products are those of stream.cuh: weights through a FIFO
+// per warp into the registers of warp MMAs, fp32 sums, 8-bit weights as exact integers.
 //
 // A slot is an expert with at most 16 of its tokens (an expert with more has several slots; the
 // second one finds the weights in L2).  The columns of its MMAs are its tokens in ascending

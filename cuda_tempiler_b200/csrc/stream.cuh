@@ -1,12 +1,13 @@
-// Products with few activation rows: each weight byte is read from HBM once, used by every row,
-// and never staged in shared memory.
+// Products with few activation rows: each weight byte is read from HBM once and used by every row.
 //
 //   y[m][n] = act(sum_k A[m][k] W[n][k] * s + bias[n]) + res[m][n],  M <= 16
 //
 // What bounds it is the weight stream (N K bytes or 2 N K bytes against 2 M K + 2 M N), so the
 // arithmetic has to cost nothing beside it: the products run on the warp tensor-core instruction
 // (m16n8k16, fp16 inputs, fp32 accumulators) with 16 weight rows as its M side and 8 activation
-// rows as its N side, operands straight from the registers the loads fill.  Sums are fp32
+// rows as its N side.  Every warp has a FIFO of its own in shared memory, filled by 16-byte
+// asynchronous copies several steps ahead (bytes in flight are what HBM needs, and registers for
+// them ran out), and reads its operands back as the registers of the MMA.  Sums are fp32
 // throughout; 8-bit weights enter as exact integers and their scale multiplies the fp32 sum (per
 // group of k, or per channel at the end), so no weight is rounded.
 //

@@ -145,8 +145,12 @@ int tempo_sm100_gemm_w8a16_swiglu(const void* A, const void* W, const void* scal
 /* GEMM with a fused epilogue: C = act(A W^T + bias) + residual, the epilogue in fp32 on the
  * accumulator and one rounding to fp16.  Layouts, strides, coverage and return codes of
  * tempo_sm100_gemm_fp16 / tempo_sm100_gemm_w8a16; workspace as
- * tempo_sm100_epilogue_workspace_bytes says (zero-filled once like the GEMMs', and interchangeable
- * with theirs; NULL runs without).
+ * tempo_sm100_epilogue_workspace_bytes says for the current device (zero-filled once like the
+ * GEMMs', and interchangeable with theirs; less, or NULL, runs without, more slowly).  Calls that
+ * can run at the same time need a workspace each.
+ * Weights: fp16 and int8 enter exactly; a group-wise weight is rounded to fp16 above 16 rows, not
+ * at all up to 16.  Up to 16 rows an infinite activation times 8-bit weights gives NaN (its sum is
+ * taken with the weights shifted by a constant), in its own row only.
  * bias: fp16 [N] or NULL.  residual: fp16 [M][N], row stride ldr elements, or NULL; it may be C
  * itself (same pointer and stride), no other overlap.  bias, residual and (W8A16) scale 16-byte
  * aligned, ldr a multiple of 8 (else 9).  activation: a TEMPO_ACT_* value (else 1). */
@@ -185,7 +189,8 @@ int tempo_sm100_moe_route(const void* x, const void* w_router, const void* bias,
  * Scales: int8 s_gate_up [E][2I], s_down [E][H]; uint8 s / z_gate_up [E][H/group][2I],
  * s / z_down [E][I/group][H].  H and I multiples of 16, group_size a multiple of 64 dividing
  * both, gu_block a multiple of 8 dividing I, top_k <= 16, E <= 512 (else 9).  residual may be y
- * itself, or NULL.  ws: tempo_sm100_moe_workspace_bytes, 16-byte aligned, any contents; calls
+ * itself, or NULL.  8-bit weights are never rounded; an infinite activation times them gives NaN,
+ * in its own token only.  ws: tempo_sm100_moe_workspace_bytes, 16-byte aligned, any contents; calls
  * that can run at the same time need one each. */
 size_t tempo_sm100_moe_workspace_bytes(int T, int top_k, int I);
 int tempo_sm100_moe_layer(const void* x, const void* w_router, const void* bias,

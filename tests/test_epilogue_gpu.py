@@ -264,6 +264,25 @@ def test_graph_capture(dev, kind, group, M):
             assert torch.equal(o, r)
 
 
+def test_linear_layers_keep_gradients(dev, monkeypatch):
+    """With gradients to record a fused layer takes the stock path, which has them."""
+    from cuda_tempiler_b200 import bind
+    monkeypatch.setenv("TEMPO_KERNELS", "1")
+    W = rand(272, 512, seed=1, scale=512 ** -0.5)
+    res, bias = rand(8, 272, seed=2), rand(272, seed=3)
+    for leaf in range(4):
+        args = [rand(8, 512, seed=4), W.clone(), bias.clone(), res.clone()]
+        args[leaf].requires_grad_()
+        bind.route_counts(reset=True)
+        y = bind.linear_fp16(args[0], args[1], args[2], activation="silu", residual=args[3])
+        assert bind.route_counts()["fallback"] == 1
+        y.sum().backward()
+        assert args[leaf].grad is not None and torch.isfinite(args[leaf].grad).all()
+        with torch.no_grad():
+            bind.linear_fp16(args[0], args[1], args[2], activation="silu", residual=args[3])
+        assert bind.route_counts()["tempo"] == 1
+
+
 def test_linear_layers_use_the_epilogue(dev, monkeypatch):
     """bind.linear_* with an activation or a residual: the kernels when they are switched on, the
     stock path otherwise, the same values within fp16's rounding."""
