@@ -254,7 +254,7 @@ def _rows(t: torch.Tensor, name: str, dtype=torch.float16) -> int:
 
 def _check_same_device(dev: torch.device, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != dev.index:
             raise ValueError(f"{name}: on {t.device}, the activations on {dev}")
 
 
@@ -329,20 +329,24 @@ def gemm_fp16_epilogue(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | No
     act, ldr = _epilogue_args(N, M, bias, activation, residual)
     dev = A.device
     _check_same_device(dev, B=B, bias=bias, residual=residual, out=out)
-    if out is not None:
+    if dev.index != torch.cuda.current_device():  # launches go to the tensors' device
+        with torch.cuda.device(dev):
+            return gemm_fp16_epilogue(A, B, bias, activation, residual, out)
+    if out is None:
+        out, ldc = A.new_empty((M, N)), N
+    else:
         _check_out(out, M, N, dev, "out")
         _check_alias(out, residual, A=A, B=B, bias=bias)
-    with _on(dev):
-        if out is None:
-            out = A.new_empty((M, N))
-        ws = None
-        if M > STREAM_MAX_M or N > STREAM_MAX_N:
-            ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, 0))
-        rc = lib.tempo_sm100_gemm_fp16_epilogue(
-            A.data_ptr(), B.data_ptr(), out.data_ptr(), _ptr(bias), _ptr(residual), M, N, K,
-            lda, ldb, out.stride(0), ldr, act, _ptr(ws), 0 if ws is None else ws.numel(),
-            _stream(dev))
-    _lib.check(rc, "tempo_sm100_gemm_fp16_epilogue")
+        ldc = out.stride(0)
+    ws, ws_bytes = None, 0
+    if M > STREAM_MAX_M or N > STREAM_MAX_N:
+        ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, 0))
+        ws_bytes = 0 if ws is None else ws.numel()
+    rc = lib.tempo_sm100_gemm_fp16_epilogue(
+        A.data_ptr(), B.data_ptr(), out.data_ptr(), _ptr(bias), _ptr(residual), M, N, K, lda, ldb,
+        ldc, ldr, act, _ptr(ws), ws_bytes, _stream(dev))
+    if rc:
+        _lib.check(rc, "tempo_sm100_gemm_fp16_epilogue")
     return out
 
 
@@ -383,20 +387,26 @@ def gemm_w8a16_epilogue(A: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
     act, ldr = _epilogue_args(N, M, bias, activation, residual)
     dev = A.device
     _check_same_device(dev, W=W, scale=scale, zero=zero, bias=bias, residual=residual, out=out)
-    if out is not None:
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return gemm_w8a16_epilogue(A, W, scale, zero, group_size, bias, activation, residual,
+                                       out)
+    if out is None:
+        out, ldc = A.new_empty((M, N)), N
+    else:
         _check_out(out, M, N, dev, "out")
         _check_alias(out, residual, A=A, W=W, scale=scale, zero=zero, bias=bias)
-    with _on(dev):
-        if out is None:
-            out = A.new_empty((M, N))
-        ws = None
-        if M > STREAM_MAX_M or N > STREAM_MAX_N:
-            ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, kind))
-        rc = lib.tempo_sm100_gemm_w8a16_epilogue(
-            A.data_ptr(), W.data_ptr(), scale.data_ptr(), _ptr(zero), out.data_ptr(), _ptr(bias),
-            _ptr(residual), M, N, K, lda, ldw, out.stride(0), ldr, kind,
-            group_size, act, _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev))
-    _lib.check(rc, "tempo_sm100_gemm_w8a16_epilogue")
+        ldc = out.stride(0)
+    ws, ws_bytes = None, 0
+    if M > STREAM_MAX_M or N > STREAM_MAX_N:
+        ws = _call_workspace(dev, lib.tempo_sm100_epilogue_workspace_bytes(M, N, K, kind))
+        ws_bytes = 0 if ws is None else ws.numel()
+    rc = lib.tempo_sm100_gemm_w8a16_epilogue(
+        A.data_ptr(), W.data_ptr(), scale.data_ptr(), _ptr(zero), out.data_ptr(), _ptr(bias),
+        _ptr(residual), M, N, K, lda, ldw, ldc, ldr, kind, group_size, act, _ptr(ws), ws_bytes,
+        _stream(dev))
+    if rc:
+        _lib.check(rc, "tempo_sm100_gemm_w8a16_epilogue")
     return out
 
 
