@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
   float* y = y_all + warp * a.T * C::YROW;
   const uint8_t* fifo_p = smem + warp * S * F::STAGE;
   const uint32_t fifo = smem_u32(fifo_p);
-  const int rot = (int)((unsigned)(nsteps * blockIdx.x) / gridDim.x);
+  const int rot = (int)((unsigned)nsteps * blockIdx.x / gridDim.x);
   // The warp's share of the sequence of all slots' steps: one run of them, so that it meets few
   // slots and adds few sums to its tokens' (steps dealt out in turn instead: one token through 8
   // int8 experts 77 us, so 71).
@@ -785,8 +785,10 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
     return (s < nsteps ? s : s - nsteps) * St::STEP;
   };
   for (int pc = 0; pc < npieces; ++pc) {
-    const int n0 = lo + (hi - lo) * pc / npieces;
-    const int n1 = lo + (hi - lo) * (pc + 1) / npieces;
+    int n0, n1;
+    split_even(hi - lo, pc, npieces, n0, n1);
+    n0 += lo;
+    n1 += lo;
     for (int i = lane; i < a.T * C::YROW; i += 32) y[i] = 0.f;
     // rows this lane's copies belong to, and where they start in an expert's matrix
     const long long row_bytes = (long long)a.I * St::ESZ;

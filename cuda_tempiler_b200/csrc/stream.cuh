@@ -89,10 +89,11 @@ __device__ __forceinline__ void stream_mma_16816(float (&d)[4], uint32_t a0, uin
 // Weights are read back by the lane that copied them.  The vectors of an activation chunk are not
 // copied by one lane each -- two lanes' copies would then touch every 32-byte sector twice (int8
 // M = 16: 77 MB of L2 traffic for 39) -- but four in a row by four lanes; blocks 16 bytes off a
-// multiple of 128 keep the reads free of bank conflicts.  Registers hold one step, the FIFO S, so the bytes in flight do not depend on how long a
-// step's arithmetic takes: with the steps in registers instead a kernel of 2 x 8 warps per SM
-// had half the bytes in flight and waited for its activations in every step (o_proj M = 1, 31 MB:
-// 12.9 us; one token through 4 fp16 experts: gate_up 35 us, down 48 us).
+// multiple of 128 keep the reads free of bank conflicts.  Registers hold one step, the FIFO S, so
+// the bytes in flight do not depend on how long a step's arithmetic takes: with the steps in
+// registers instead a kernel of 2 x 8 warps per SM had half the bytes in flight and waited for its
+// activations in every step (o_proj M = 1, 31 MB: 12.9 us, so 6.6; one token through 4 fp16
+// experts: gate_up 35 us, so 20, down 48, so 12).
 // ---------------------------------------------------------------------------------------------
 template <int WQ, int MG, int RT, int BV>
 struct StreamFifo {
@@ -295,7 +296,7 @@ __device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red_
   typename Job::Piece lp, up;
   const int n_mine = nsteps > warp ? ((nsteps - 1 - warp) >> (31 - __clz(KS))) + 1 : 0;
   bool more = n_mine > 0 && job.first(lp);
-  const int rot = Job::ROTATE ? (int)((unsigned)(nsteps * wk.id) / (unsigned)wk.count) : 0;
+  const int rot = Job::ROTATE ? (int)((unsigned)nsteps * (unsigned)wk.id / (unsigned)wk.count) : 0;
   int lstep = warp, lslot = 0;
   auto issue = [&]() {
     if (more) {
@@ -396,8 +397,9 @@ struct LinearJob {
     GroupWord z[WQ == kWUint8Group ? RT : 1];
   };
   __device__ __forceinline__ void bounds(Piece& p) const {
-    p.n0 = lo + (hi - lo) * p.i / npieces;
-    p.n1 = lo + (hi - lo) * (p.i + 1) / npieces;
+    split_even(hi - lo, p.i, npieces, p.n0, p.n1);
+    p.n0 += lo;
+    p.n1 += lo;
     p.w = a.W + ((long long)(p.n0 + (lane >> 2)) * a.ldw + (lane & 3) * St::KC) * St::ESZ;
     if (WQ == kWUint8Group) {
 #pragma unroll
