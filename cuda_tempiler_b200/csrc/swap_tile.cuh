@@ -7,17 +7,26 @@
 //
 // so every weight byte is read from HBM by exactly one CTA and used for all of M; the 128 x M fp32
 // accumulator stays in TMEM.  The activations (M x 128 bytes per k-block) come from L2 by TMA once
-// per weight tile.
+// per weight tile.  (8-bit weights of more rows: tiles of up to 384 of them, a weight tile's one
+// after the other.)
 //
-// 8-bit weights: raw tiles in a ring of their own (released as soon as they are unpacked, so that the
-// HBM latency hides behind more bytes than the fp16 slots could hold); eight warps turn them into
-// the slot's swizzled fp16 operand: int8 exactly (the channel's scale multiplies the fp32 sum),
+// What bounds it: up to 128 rows the weights from HBM and 400 (fp16) to 500 (8-bit) cycles that a
+// k-block's chain of barriers and MMA issue takes; above, the activations' way from L2, 40 B per
+// cycle and SM.  Measured (us, floor in brackets): fp16 17 x 15360 x 3840 21.4 (18.2),
+// 100 x 15360 x 3840 24.0 (18.7), 256 x 18944 x 3840 36.5 (24.1), 333 x 18944 x 3840 45.5 (28.9);
+// int8 100 x 15360 x 3840 22.8 (9.6); uint8 333 x 5120 x 17408 62 (35.4), 51 of it here, the rest
+// k_swap_finish.  (A pair of CTAs per tile, cta_group::2 with half the activations each: the same
+// with fp16 weights, up to twice as long with 8-bit ones.)
+//
+// 8-bit weights: raw tiles in a ring of their own (released as soon as they are unpacked, so that
+// the HBM latency hides behind more bytes than the fp16 slots could hold); eight warps turn them
+// into the slot's swizzled fp16 operand: int8 exactly (the channel's scale multiplies the sum),
 // group-wise (q - z) * s rounded once to fp16, the only form the tensor core takes.  (Weights by
 // plain loads into a register ring instead of TMA: 500 cycles of one warp's time per k-block for
 // eight loads and their addresses, 100 x 15360 x 3840 42 us.)
 //
 // Work split: the k-blocks of all weight tiles are one sequence, cut into equal contiguous shares,
-// one per CTA, unless whole tiles fill the GPU well enough (epi_swap_plan).  A share starts and
+// one per CTA, unless whole tiles fill the GPU well enough (epi_swap_cost).  A share starts and
 // ends inside a tile: the fp32 sums of such partial tiles go to the workspace and k_swap_finish,
 // one launch behind, adds them in k order and applies the epilogue with every SM (the last CTA to
 // arrive doing so alone took 20 us for 5 parts of a 128 x 128 tile).  No CTA waits for another.
@@ -64,7 +73,7 @@ constexpr int kSwapMaxSlots = 8;
 
 struct SwapArgs {
   int M, N, num_kb;
-  int tiles, mt;              // tile t: weight rows 128 (t / mt) .., activation rows rows (t % mt) ..
+  int tiles, mt;              // tile t: weight rows from 128 (t / mt), activations from rows (t % mt)
   int rows;                   // activation rows of a tile: n groups
   int n, groups;              // rows per MMA (multiple of 16), MMAs per k step
   int nx, nr;                 // operand slots, raw tiles
@@ -148,8 +157,8 @@ struct EpiCols {
 template <int WQ>
 constexpr int kSwapThreads = WQ ? 19 * 32 : 10 * 32;
 
-// LG: groups of unpacking warps.  2: four warps fill a slot, the others the next one (a slot's turn,
-// its data, the fence and the arrival take a warp longer than a k-block of 8-bit weights may); a
+// LG: groups of unpacking warps.  2: four warps fill a slot, the others the next one (a slot's
+// turn, its data, the fence and the arrival take a warp longer than a k-block may); a
 // slot and a raw tile then always have the same group, so nx and nr are even.  1: all eight fill
 // every slot.
 template <int WQ, int LG>
@@ -280,8 +289,8 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA
-    // The whole warp runs the loop, so that descriptors and barrier addresses stay uniform; one lane
-    // issues.  (All of it in one lane: 550 cycles for a k-block's four MMAs, whatever their width.)
+    // The whole warp runs the loop, so that descriptors and barrier addresses stay uniform; one
+    // lane issues.  (All of it in one lane: 550 cycles for a k-block's four MMAs, so 210.)
     const uint32_t idesc = idesc_f16_f32(128, a.n);
     // sdesc_k_sw128 split into its words: only the low one changes
     const uint32_t hi = (uint32_t)(sdesc_k_sw128(0) >> 32);
@@ -555,7 +564,8 @@ double epi_swap_cost(SwapPlan& p, int wkind, int M, int N, int K, int sms, size_
     }
     if (p.epis == 1 || p.nx > 2) break;
   }
-  p.smem = 1024 + p.nx * p.x_bytes + p.nr * kSwapRawBytes + p.epis * kSwapStageBytes + kSwapBarBytes;
+  p.smem = 1024 + p.nx * p.x_bytes + p.nr * kSwapRawBytes + p.epis * kSwapStageBytes +
+           kSwapBarBytes;
   const double wb = 128.0 * 64 * (wkind == 0 ? 2 : 1) / p.mt;
   auto kb_cycles = [&](int active) {
     return std::max({p.groups * 4.0 * std::max(45.0, p.n / 2.0), p.rows * 128.0 / 64.0, wb / 30.0,

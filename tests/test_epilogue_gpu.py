@@ -283,6 +283,27 @@ def test_linear_layers_keep_gradients(dev, monkeypatch):
         assert bind.route_counts()["tempo"] == 1
 
 
+def test_calls_at_the_same_time(dev):
+    """Calls on several streams at once, each with the workspace of its stream: shares of k whose
+    parts meet there, split tails with their counters."""
+    shapes = [("fp16", 0, 90, 784, 4096), ("uint8", 128, 300, 528, 4096), ("fp16", 0, 512, 3840, 4096)]
+    jobs = []
+    for i, (kind, group, M, N, K) in enumerate(shapes):
+        A, w, res = rand(M, K, seed=i), weights(kind, N, K, group, seed=i), rand(M, N, seed=9 + i)
+        jobs.append((A, w, group, res, call(A, w, group, residual=res)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for _ in range(6):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append([call(A, w, group, residual=res) for A, w, group, res, _ in jobs])
+    torch.cuda.synchronize()
+    for ys in got:
+        for y, job in zip(ys, jobs):
+            assert torch.equal(y, job[4])
+
+
 def test_linear_layers_use_the_epilogue(dev, monkeypatch):
     """bind.linear_* with an activation or a residual: the kernels when they are switched on, the
     stock path otherwise, the same values within fp16's rounding."""
