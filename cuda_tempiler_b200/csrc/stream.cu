@@ -15,7 +15,8 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool aligned16(const void* p) { return aligned(p, 16); }
 
 int current_sms() {
   static int sms[kMaxDevices];
@@ -126,12 +127,13 @@ cudaError_t run_stream(const LinearArgs& a, int wkind, cudaStream_t st) {
 namespace tempo_sm100 {
 namespace {
 
-int route_args(const void* x, const void* wr, const int* ids, const float* weights, int T, int E,
-               int H, int k, int ldx, int ldw) {
+int route_args(const void* x, const void* wr, const void* bias, const int* ids,
+               const float* weights, int T, int E, int H, int k, int ldx, int ldw) {
   if (!x || !wr || !ids || !weights || T < 1 || E < 1 || H < 1 || k < 1 || k > E)
     return cudaErrorInvalidValue;
   if (E > kMoeMaxE || k > kMoeMaxK || H % 8 || ldx < H || ldw < H || ldx % 8 || ldw % 8 ||
-      !aligned16(x) || !aligned16(wr))
+      !aligned16(x) || !aligned16(wr) || !aligned(bias, 2) || !aligned(ids, 4) ||
+      !aligned(weights, 4))
     return cudaErrorInvalidConfiguration;
   return 0;
 }
@@ -146,7 +148,14 @@ int moe_args(MoeArgs& a, const void* x, const void* wgu, const void* wd, const v
       (kind == kWUint8Group && (!zgu || !zd)))
     return cudaErrorInvalidValue;
   if (T > kMoeMaxT || E > kMoeMaxE || k > kMoeMaxK || H % 16 || I % 16 || ldx < H || ldx % 8 ||
-      ldy < H || (res && ldr < H) || !aligned16(x) || !aligned16(wgu) || !aligned16(wd))
+      ldy < H || (res && ldr < H) || !aligned16(x) || !aligned16(wgu) || !aligned16(wd) ||
+      !aligned(res, 2) || !aligned(y, 2))
+    return cudaErrorInvalidConfiguration;
+  // group-wise scales and zero points are copied in 4-byte words (copy_group_word), a channel's
+  // scale is read by itself
+  const unsigned word = kind == kWUint8Group ? 4 : 2;
+  if (kind && (!aligned(sgu, word) || !aligned(sd, word))) return cudaErrorInvalidConfiguration;
+  if (kind == kWUint8Group && (!aligned(zgu, word) || !aligned(zd, word)))
     return cudaErrorInvalidConfiguration;
   if (kind == kWUint8Group && (group <= 0 || group % 64 || H % group || I % group))
     return cudaErrorInvalidConfiguration;
@@ -187,7 +196,7 @@ extern "C" {
 int tempo_sm100_moe_route(const void* x, const void* w_router, const void* bias, int* ids,
                           float* weights, int T, int E, int H, int top_k, int ldx, int ldw,
                           int normalize, void* stream) {
-  const int rc = route_args(x, w_router, ids, weights, T, E, H, top_k, ldx, ldw);
+  const int rc = route_args(x, w_router, bias, ids, weights, T, E, H, top_k, ldx, ldw);
   if (rc) return rc;
   return launch_route({static_cast<const __half*>(x), ldx, static_cast<const __half*>(w_router),
                        ldw, static_cast<const __half*>(bias), T, E, H, top_k, normalize, ids,
@@ -207,7 +216,7 @@ int tempo_sm100_moe_layer(const void* x, const void* w_router, const void* bias,
                           int H, int I, int top_k, int ldx, int ldw, int ldr, int ldy,
                           int weight_kind, int group_size, int gu_block, int normalize, void* ws,
                           size_t ws_bytes, void* stream) {
-  int rc = route_args(x, w_router, ids, weights, T, E, H, top_k, ldx, ldw);
+  int rc = route_args(x, w_router, bias, ids, weights, T, E, H, top_k, ldx, ldw);
   if (rc) return rc;
   MoeArgs a{};
   rc = moe_args(a, x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, residual, y, T, E,
@@ -229,6 +238,7 @@ int tempo_sm100_moe_experts(const void* x, const int* ids, const float* weights,
                             int ldx, int ldr, int ldy, int weight_kind, int group_size,
                             int gu_block, void* ws, size_t ws_bytes, void* stream) {
   if (!ids || !weights) return cudaErrorInvalidValue;
+  if (!aligned(ids, 4) || !aligned(weights, 4)) return cudaErrorInvalidConfiguration;
   MoeArgs a{};
   const int rc =
       moe_args(a, x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, residual, y, T, E,

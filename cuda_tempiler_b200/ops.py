@@ -499,7 +499,8 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor,
     over each token's experts.  w_gate_up [E, 2I, H] holds gate rows then up rows (gu_block 0) or
     alternates them in blocks of gu_block; w_down [E, H, I].  fp16, int8 with a scale per output
     channel (s_gate_up [E, 2I], s_down [E, H]) or uint8 with scale and zero point per group
-    ([E, H / group_size, 2I], [E, I / group_size, H]).  ``out`` may be ``residual``.  Returns y, or
+    ([E, H / group_size, 2I], [E, I / group_size, H]), both 4-byte aligned (else NotCovered).
+    ``out`` may be ``residual``.  Returns y, or
     (y, ids, weights) with return_routing."""
     lib = _lib.load()
     T, H, E, I, kind, ldr = _check_experts(x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down,

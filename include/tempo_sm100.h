@@ -188,7 +188,8 @@ int tempo_sm100_moe_route(const void* x, const void* w_router, const void* bias,
  * b > 0: gate and up rows alternate in blocks of b (as tempo_sm100_silu_mul's columns).
  * Scales: int8 s_gate_up [E][2I], s_down [E][H]; uint8 s / z_gate_up [E][H/group][2I],
  * s / z_down [E][I/group][H].  H and I multiples of 16, group_size a multiple of 64 dividing
- * both, gu_block a multiple of 8 dividing I, top_k <= 16, E <= 512 (else 9).  residual may be y
+ * both, gu_block a multiple of 8 dividing I, top_k <= 16, E <= 512; x and both weights 16-byte
+ * aligned, group-wise scales and zero points 4-byte aligned (else 9).  residual may be y
  * itself, or NULL.  8-bit weights are never rounded; an infinite activation times them gives NaN,
  * in its own token only.  ws: tempo_sm100_moe_workspace_bytes, 16-byte aligned, any contents; calls
  * that can run at the same time need one each. */

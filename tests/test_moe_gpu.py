@@ -417,3 +417,27 @@ def test_tensor_parallel_helpers(dev, kind, M):
     total = parts[0].double() + parts[1].double()
     assert ((total - ref).abs() <= 2 * tol + 2.0 ** -10 * (parts[1].double().abs() +
                                                           parts[0].double().abs())).all()
+
+
+def test_packed_scales_and_zero_points(dev):
+    """Scales and zero points as views into one buffer: taken at any word, refused off one."""
+    from cuda_tempiler_b200 import ops
+    ly = Layer("uint8", 6, 128, 192, 64, seed=110)
+    x = whole(5, 128, seed=111)
+    want = ly(x, 3)
+
+    def at(t, off):  # t's values from `off` elements behind a 16-byte boundary
+        buf = torch.empty(t.numel() + 16, dtype=t.dtype, device="cuda")
+        return buf[off:off + t.numel()].view(t.shape).copy_(t)
+
+    gu, dn = ly.gu, ly.dn
+    ly.gu, ly.dn = (gu[0], at(gu[1], 2), at(gu[2], 4)), (dn[0], at(dn[1], 6), at(dn[2], 12))
+    assert torch.equal(ly(x, 3), want)
+    for i, off in ((1, 1), (1, 3), (2, 1), (2, 2), (2, 3)):
+        for which in "gu", "dn":
+            ly.gu, ly.dn = gu, dn
+            w = list(getattr(ly, which))
+            w[i] = at(w[i], off)
+            setattr(ly, which, w)
+            with pytest.raises(ops.NotCovered):
+                ly(x, 3)

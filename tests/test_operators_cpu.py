@@ -89,6 +89,28 @@ def test_layer_refuses(kw, rc):
     assert layer(**kw) == rc
 
 
+@pytest.mark.parametrize("name", ["sgu", "zgu", "sd", "zd"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_group_scales_off_a_word_are_refused(name, off):
+    """The experts read group-wise scales and zero points in 4-byte words."""
+    assert layer(**{name: P + off}) == NOT_COVERED
+    assert layer(**{name: P + 4, "ws": None}) == BAD  # a word's boundary passes that check
+    a = dict(x=P, ids=P, w=P, wgu=P, wd=P, sgu=P, zgu=P, sd=P, zd=P, res=None, y=P, T=4, E=16,
+             H=128, I=128, k=2, ldx=128, ldr=0, ldy=128, kind=2, group=64, block=0, ws=P,
+             ws_bytes=1 << 30)
+    a[name] += off
+    assert lib().tempo_sm100_moe_experts(*a.values(), None) == NOT_COVERED
+
+
+@pytest.mark.parametrize("kw", [dict(res=P + 1, ldr=128), dict(y=P + 1), dict(bias=P + 1),
+                                dict(ids=P + 2), dict(w=P + 2), dict(kind=1, sgu=P + 1),
+                                dict(kind=1, sd=P + 1)])
+def test_elements_off_their_own_size_are_refused(kw):
+    assert layer(**kw) == NOT_COVERED
+    kw = {n: v for n, v in kw.items() if n in ("bias", "ids", "w")}
+    assert not kw or route(**kw) == NOT_COVERED
+
+
 def test_experts_refuse():
     def experts(**kw):
         a = dict(x=P, ids=P, w=P, wgu=P, wd=P, sgu=None, zgu=None, sd=None, zd=None, res=None, y=P,
