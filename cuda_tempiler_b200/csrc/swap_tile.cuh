@@ -55,6 +55,14 @@ __device__ __forceinline__ bool named_barrier_and(int id, int threads, bool p) {
   return r != 0;
 }
 
+// A bounded wait of a whole warp.  It may run out, or see the abort flag, in some lanes only: the
+// warp goes on or gives up as one, since what follows takes all of its lanes (elect.sync,
+// __syncwarp).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                          int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, where));
+}
+
 // True in one lane of a converged warp, always the same one.
 __device__ __forceinline__ bool elect_one() {
   uint32_t one;
@@ -301,12 +309,12 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
     bool ok = true;
     for (; ok && segs.next(sg); ++lu) {
       const int buf = lu % a.bufs;
-      if (!mbar_wait(tempty(buf), (uint32_t)((lu / a.bufs) & 1) ^ 1u, abort_flag, 33)) break;
+      if (!warp_wait(tempty(buf), (uint32_t)((lu / a.bufs) & 1) ^ 1u, abort_flag, 33)) break;
       tc_fence_after();
       const uint32_t d = tmem_base + buf * 256;
       uint32_t add = 0;
       for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
-        if (!mbar_wait(xfull(s), ph, abort_flag, 34)) {
+        if (!warp_wait(xfull(s), ph, abort_flag, 34)) {
           ok = false;
           break;
         }
@@ -425,7 +433,7 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
     int s = grp, r = grp;
     uint32_t ph = 1, rph = 0;
     for (int it = grp; it < n_its; it += LG) {
-      if (!mbar_wait(rfull(r), rph, abort_flag, 37)) break;
+      if (!warp_wait(rfull(r), rph, abort_flag, 37)) break;
       const uint8_t* src = raw + r * kSwapRawBytes;
       uint4 x[L];
       __half2 zb[L], s2[L];
@@ -439,7 +447,7 @@ __global__ void __launch_bounds__(kSwapThreads<WQ>, 1)
           s2[i] = __half2half2(reinterpret_cast<const __half*>(src + 8192)[wr]);
         }
       }
-      if (!mbar_wait(xempty(s), ph, abort_flag, 38)) break;
+      if (!warp_wait(xempty(s), ph, abort_flag, 38)) break;
       uint8_t* dst = smem + s * a.x_bytes + R * d * 128;
 #pragma unroll
       for (int i = 0; i < L; ++i) {

@@ -162,6 +162,29 @@ def test_stock_path_of_the_linear_layers():
         bind.linear_fp16(x, w, activation="tanh", residual=r)
 
 
+def test_whole_warps_give_up_together():
+    """Where all lanes of a warp wait and then act as a warp, the wait's outcome is the warp's
+    (warp_wait) or the barrier group's (named_barrier_and); a lane that waits by itself does so
+    under `lane == 0`."""
+    import re
+    from pathlib import Path
+
+    import cuda_tempiler_b200
+    text = (Path(cuda_tempiler_b200.__file__).parent / "csrc" / "swap_tile.cuh").read_text()
+    kernel = text[text.index("k_epi_swap(const __grid_constant__"):text.index("k_swap_finish(const")]
+    parts = re.split(r"// -{20,} (.*)\n", kernel)
+    roles = dict(zip(parts[1::2], parts[2::2]))
+    assert list(roles) == ["TMA", "TMA: raw weights", "MMA", "epilogue", "unpacking"]
+    for name, body in roles.items():
+        waits = re.findall(r"(\w*\(?\w*, ?\w*, ?)?\bmbar_wait\(", body)
+        if name.startswith("TMA"):
+            assert body.lstrip().startswith("if (lane == 0) {") and len(waits) == 1
+        elif name == "epilogue":
+            assert len(waits) == 1 and "named_barrier_and(bar, 128, mbar_wait(" in body
+        else:
+            assert not waits and "warp_wait(" in body, name
+
+
 # ------------------------------------------------------------------------------ sharding
 def _port():
     s = socket.socket()
