@@ -921,11 +921,8 @@ __global__ void __launch_bounds__(32 * DownCfg<WQ, MG, RT>::NW, 1)
               b[1][2 * v + i] = fin[mg] ? *reinterpret_cast<const uint32_t*>(&lo2) : 0u;
             }
           }
-          float bias[4];
-          stream_bias<WQ>(b, bias);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            stream_mma<WQ, RT, false>(w, rt, b, bias, acc[rt][mg]);
+          for (int rt = 0; rt < RT; ++rt) stream_mma<WQ, RT, false>(w, rt, b, acc[rt][mg]);
         }
         ufifo = ufifo + 1 == S ? 0 : ufifo + 1;
         advance(u);

@@ -39,14 +39,17 @@ struct StreamStep {
   static constexpr int NB = KC / 2;        // 32-bit registers of one activation chunk
 };
 
-// The fp16 operands of a chunk in storage order: fp16 weights as they are; 8-bit weights as
-// 1024 + u, exact, with u the unsigned byte (int8 q: u = q + 128).  What that adds to a step's sum,
-// (1024 + 128 or z) x the sum of the step's activations, is taken off the sum instead of every
-// weight: the activations' sum is one more chain of MMAs for all row tiles together, the
-// subtraction from every weight half of the unpacking.  A step's sum is at most 64 products, so
-// what the cancellation costs (its terms are about 16 times the difference's) is some 2^-18 of it.
+// The fp16 operands of a chunk in storage order: fp16 weights as they are; 8-bit weights as the
+// integers they stand for, q or q - z (8 magnitude bits: exact in fp16).  A byte in the low half of
+// 0x6400 is 1024 + u with u the unsigned byte (int8 q: u = q + 128); what has to go, `off` = 1152 or
+// 1024 + z, is subtracted from every weight, two at a time.  (Left in and taken off the step's sum
+// instead, by an MMA chain over the activations alone: the sum then passes through values 1152 / |q|
+// times its own, of which a tensor core truncates the low bits, always in the same direction where
+// the activations have one sign.  With weights of +-3 results were off by up to 25 times the bound
+// that the exact operands keep, and no faster: one token through 8 int8 experts 69.9 us, so 68.9.)
 template <int WQ>
-__device__ __forceinline__ void stream_unpack(uint4 x, uint32_t (&h)[StreamStep<WQ>::NB]) {
+__device__ __forceinline__ void stream_unpack(uint4 x, uint32_t (&h)[StreamStep<WQ>::NB],
+                                              __half2 off) {
   if constexpr (WQ == kWFp16) {
     h[0] = x.x;
     h[1] = x.y;
@@ -56,27 +59,22 @@ __device__ __forceinline__ void stream_unpack(uint4 x, uint32_t (&h)[StreamStep<
     const uint32_t flip = WQ == kWInt8PerChannel ? 0x80808080u : 0u;
     const uint32_t v[4] = {x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h[2 * i] = __byte_perm(v[i], 0x64646464u, 0x5150);
-      h[2 * i + 1] = __byte_perm(v[i], 0x64646464u, 0x5352);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = __byte_perm(v[i >> 1], 0x64646464u, i & 1 ? 0x5352 : 0x5150);
+      const __half2 w = __hsub2(*reinterpret_cast<const __half2*>(&u), off);
+      h[i] = *reinterpret_cast<const uint32_t*>(&w);
     }
   }
 }
 
-// d = a x b + c (not volatile: the compiler may move it)
-__device__ __forceinline__ void stream_mma_16816(float (&d)[4], uint32_t a0, uint32_t a1,
-                                                 uint32_t a2, uint32_t a3, uint32_t b0,
-                                                 uint32_t b1, float c0, float c1, float c2,
-                                                 float c3) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%10,%11,%12,%13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
-}
+// d += a x b (not volatile: the compiler may move it)
 __device__ __forceinline__ void stream_mma_16816(float (&d)[4], uint32_t a0, uint32_t a1,
                                                  uint32_t a2, uint32_t a3, uint32_t b0,
                                                  uint32_t b1) {
-  stream_mma_16816(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -160,9 +158,9 @@ __device__ __forceinline__ void copy_group_word(uint32_t dst, const GroupWord& w
 
 // Scale and 1024 + zero point of `row` of the tile.
 __device__ __forceinline__ void read_group_row(const uint8_t* src, int r0, int row, float& s,
-                                               float& zb) {
+                                               __half2& off) {
   s = __half2float(*reinterpret_cast<const __half*>(src + 2 * ((r0 & 1) + row)));
-  zb = __half2float(
+  off = __half2half2(
       __ushort_as_half((unsigned short)(0x6400u | src[4 * kZeroLane + (r0 & 3) + row])));
 }
 
@@ -170,9 +168,7 @@ __device__ __forceinline__ void read_group_row(const uint8_t* src, int r0, int r
 template <int WQ, int RT>
 struct StreamA {
   uint32_t a[RT][StreamStep<WQ>::NB], b[RT][StreamStep<WQ>::NB];
-  // group-wise: scale and 1024 + zero point of the two rows
   float fa[WQ == kWUint8Group ? RT : 1], fb[WQ == kWUint8Group ? RT : 1];
-  float za[WQ == kWUint8Group ? RT : 1], zb[WQ == kWUint8Group ? RT : 1];
 };
 
 template <int WQ, int RT>
@@ -183,67 +179,42 @@ __device__ __forceinline__ void stream_read_weights(StreamA<WQ, RT>& o, const ui
   for (int rt = 0; rt < RT; ++rt) {
     const uint4 xa = lds16(stage + rt * 1024 + lane * 16);
     const uint4 xb = lds16(stage + rt * 1024 + 512 + lane * 16);
+    __half2 za = __half2half2(__ushort_as_half(0x6480)), zb = za;  // 1152
     if constexpr (WQ == kWUint8Group) {
-      read_group_row(stage + z_off + rt * 128, z_row[rt], lane >> 2, o.fa[rt], o.za[rt]);
-      read_group_row(stage + z_off + rt * 128, z_row[rt], (lane >> 2) + 8, o.fb[rt], o.zb[rt]);
+      read_group_row(stage + z_off + rt * 128, z_row[rt], lane >> 2, o.fa[rt], za);
+      read_group_row(stage + z_off + rt * 128, z_row[rt], (lane >> 2) + 8, o.fb[rt], zb);
     }
-    stream_unpack<WQ>(xa, o.a[rt]);
-    stream_unpack<WQ>(xb, o.b[rt]);
+    stream_unpack<WQ>(xa, o.a[rt], za);
+    stream_unpack<WQ>(xb, o.b[rt], zb);
   }
 }
 
-// What stream_mma subtracts for a step's activation chunks b (N of them: their values add up):
-// int8: -1152 x the sum of each column (d[0], d[1]: columns 2t, 2t + 1); uint8: the sum itself.
-template <int WQ, int N>
-__device__ __forceinline__ void stream_bias(const uint32_t (&b)[N][StreamStep<WQ>::NB],
-                                            float (&d)[4]) {
-  if constexpr (WQ != kWFp16) {
-    const uint32_t c = WQ == kWInt8PerChannel ? 0xE480E480u : 0x3C003C00u;  // -1152 or 1
-    stream_mma_16816(d, c, c, c, c, b[0][0], b[0][1], 0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int j = n ? 0 : 1; j < StreamStep<WQ>::NMMA; ++j)
-        stream_mma_16816(d, c, c, c, c, b[n][2 * j], b[n][2 * j + 1]);
-  }
-}
-
-// acc += weights of row tile rt x the step's activation chunks.  The step's sum starts at zero (or
-// at its bias) and is added in fp32, except (STEPS false) for fp16 weights: a tensor core truncates
-// what it adds to a large accumulator, which over a long K shows in fp32 results, not in fp16 ones.
+// acc += weights of row tile rt x the step's activation chunks b (N of them: their values add up).
+// The step's sum starts at zero and is added in fp32 (group-wise: times the scale), except (STEPS
+// false) for fp16 weights: a tensor core truncates what it adds to a large accumulator, which over
+// a long K shows in fp32 results, not in fp16 ones.
 template <int WQ, int RT, bool STEPS, int N>
 __device__ __forceinline__ void stream_mma(const StreamA<WQ, RT>& w, int rt,
                                            const uint32_t (&b)[N][StreamStep<WQ>::NB],
-                                           const float (&bias)[4], float (&acc)[4]) {
+                                           float (&acc)[4]) {
   using S = StreamStep<WQ>;
-  if constexpr (WQ != kWFp16 || STEPS) {
-    float d[4];
-    const bool from = WQ == kWInt8PerChannel;
-    stream_mma_16816(d, w.a[rt][0], w.b[rt][0], w.a[rt][1], w.b[rt][1], b[0][0], b[0][1],
-                from ? bias[0] : 0.f, from ? bias[1] : 0.f, from ? bias[2] : 0.f,
-                from ? bias[3] : 0.f);
+  constexpr bool own = WQ != kWFp16 || STEPS;
+  float step[4] = {};
+  float(&d)[4] = own ? step : acc;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int j = n ? 0 : 1; j < S::NMMA; ++j)
-        stream_mma_16816(d, w.a[rt][2 * j], w.b[rt][2 * j], w.a[rt][2 * j + 1], w.b[rt][2 * j + 1],
-                  b[n][2 * j], b[n][2 * j + 1]);
-    if constexpr (WQ == kWUint8Group) {
-      acc[0] = fmaf(fmaf(-w.za[rt], bias[0], d[0]), w.fa[rt], acc[0]);
-      acc[1] = fmaf(fmaf(-w.za[rt], bias[1], d[1]), w.fa[rt], acc[1]);
-      acc[2] = fmaf(fmaf(-w.zb[rt], bias[0], d[2]), w.fb[rt], acc[2]);
-      acc[3] = fmaf(fmaf(-w.zb[rt], bias[1], d[3]), w.fb[rt], acc[3]);
-    } else {
+    for (int j = 0; j < S::NMMA; ++j)
+      stream_mma_16816(d, w.a[rt][2 * j], w.b[rt][2 * j], w.a[rt][2 * j + 1], w.b[rt][2 * j + 1],
+                       b[n][2 * j], b[n][2 * j + 1]);
+  if constexpr (WQ == kWUint8Group) {
+    acc[0] = fmaf(d[0], w.fa[rt], acc[0]);
+    acc[1] = fmaf(d[1], w.fa[rt], acc[1]);
+    acc[2] = fmaf(d[2], w.fb[rt], acc[2]);
+    acc[3] = fmaf(d[3], w.fb[rt], acc[3]);
+  } else if constexpr (own) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] += d[i];
-    }
-  } else {
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int j = 0; j < S::NMMA; ++j)
-        stream_mma_16816(acc, w.a[rt][2 * j], w.b[rt][2 * j], w.a[rt][2 * j + 1], w.b[rt][2 * j + 1],
-                  b[n][2 * j], b[n][2 * j + 1]);
+    for (int i = 0; i < 4; ++i) acc[i] += d[i];
   }
 }
 
@@ -340,10 +311,8 @@ __device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red_
           b[0][4 * v + 2] = x.z;
           b[0][4 * v + 3] = x.w;
         }
-        float bias[4];
-        stream_bias<WQ>(b, bias);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) stream_mma<WQ, RT, STEPS>(w, rt, b, bias, acc[rt][mg]);
+        for (int rt = 0; rt < RT; ++rt) stream_mma<WQ, RT, STEPS>(w, rt, b, acc[rt][mg]);
       }
       slot = slot + 1 == S ? 0 : slot + 1;
     }

@@ -149,8 +149,7 @@ int tempo_sm100_gemm_w8a16_swiglu(const void* A, const void* W, const void* scal
  * GEMMs', and interchangeable with theirs; less, or NULL, runs without, more slowly).  Calls that
  * can run at the same time need a workspace each.
  * Weights: fp16 and int8 enter exactly; a group-wise weight is rounded to fp16 above 16 rows, not
- * at all up to 16.  Up to 16 rows an infinite activation times 8-bit weights gives NaN (its sum is
- * taken with the weights shifted by a constant), in its own row only.
+ * at all up to 16.  An infinite activation makes its own row infinite (NaN where the weight is 0).
  * bias: fp16 [N] or NULL.  residual: fp16 [M][N], row stride ldr elements, or NULL; it may be C
  * itself (same pointer and stride), no other overlap.  bias, residual and (W8A16) scale 16-byte
  * aligned, ldr a multiple of 8 (else 9).  activation: a TEMPO_ACT_* value (else 1). */
@@ -190,7 +189,7 @@ int tempo_sm100_moe_route(const void* x, const void* w_router, const void* bias,
  * s / z_down [E][I/group][H].  H and I multiples of 16, group_size a multiple of 64 dividing
  * both, gu_block a multiple of 8 dividing I, top_k <= 16, E <= 512; x and both weights 16-byte
  * aligned, group-wise scales and zero points 4-byte aligned (else 9).  residual may be y
- * itself, or NULL.  8-bit weights are never rounded; an infinite activation times them gives NaN,
+ * itself, or NULL.  8-bit weights are never rounded; an infinite activation leaves nothing finite
  * in its own token only.  ws: tempo_sm100_moe_workspace_bytes, 16-byte aligned, any contents; calls
  * that can run at the same time need one each. */
 size_t tempo_sm100_moe_workspace_bytes(int T, int top_k, int I);

@@ -370,3 +370,59 @@ def test_refusals(dev):
         ops.gemm_fp16_epilogue(A, rand(44, 64))
     with pytest.raises(ops.NotCovered):
         ops.gemm_fp16_epilogue(A[:0], B)
+
+
+def narrow(kind, N, K, group, seed=0):
+    """8-bit weights of a few steps around zero (one outlier of the channel or group has set the
+    scale), the zero points anywhere."""
+    g = torch.Generator("cuda").manual_seed(seed + 2000)
+    q = torch.randint(-3, 4, (N, K), generator=g, device="cuda", dtype=torch.int16)
+    if kind == "int8":
+        return q.to(torch.int8), ((torch.rand(N, generator=g, device="cuda") + 0.5) * 0.01).half(), \
+            None
+    z = torch.randint(3, 253, (K // group, N), generator=g, device="cuda", dtype=torch.int16)
+    W = (q + z.repeat_interleave(group, 0).t()).to(torch.uint8)
+    s = ((torch.rand(K // group, N, generator=g, device="cuda") + 0.5) * 0.01).half()
+    return W, s, z.to(torch.uint8)
+
+
+@pytest.mark.parametrize("kind,group", [("int8", 0), ("uint8", 64), ("uint8", 128)])
+@pytest.mark.parametrize("M", [1, 8, 16])
+@pytest.mark.parametrize("K", [1024, 4096, 16384])
+def test_one_signed_activations_times_narrow_weights(dev, kind, group, M, K):
+    """Up to 16 rows the products of an 8-bit weight enter the sum as they are: nothing in it is
+    larger than S = sum |a| |w|.  A warp's step adds 4 times 16 products on the tensor core (20
+    truncations of at most 2^-23 S at the most), the K / 1024 steps of a warp and the 16 warps are
+    added in fp32."""
+    N = 272
+    A, w = rand(M, K, seed=M).abs(), narrow(kind, N, K, group, seed=K)
+    y = call(A, w, group)
+    Wd = L.dequant(*w, group)
+    ref, S = A.double() @ Wd.t(), A.double() @ Wd.abs().t()
+    tol = (20 + K / 1024 + 16) * 2.0 ** -23 * S
+    tol = tol + L.U16 * (ref.abs() + tol) + 2.0 ** -25
+    bad = ~((y.double() - ref).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), float(((y.double() - ref).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("kind,group", [("int8", 0), ("uint8", 64)])
+def test_an_infinite_activation_times_8_bit_weights(dev, kind, group):
+    """Its row is infinite with the sign of the weight, NaN where the weight is zero, on every path."""
+    N, K = 272, 512
+    W, s, z = weights(kind, N, K, group)
+    if kind == "int8":
+        W[:, 7] = torch.arange(N, device="cuda").remainder(3).sub(1).to(torch.int8)
+    else:
+        W[:, 7] = (z[0].int().clamp(1, 254) + torch.arange(N, device="cuda") % 3 - 1).to(torch.uint8)
+        z[0] = z[0].clamp(1, 254)
+    sign = torch.arange(N, device="cuda") % 3 - 1
+    for M in (1, 4, 16, 40):
+        A = rand(M, K, seed=M)
+        clean = call(A, (W, s, z), group)
+        A[M // 2, 7] = float("inf")
+        y = call(A, (W, s, z), group)
+        row = y[M // 2].float()
+        assert torch.isnan(row[sign == 0]).all()
+        assert (row[sign > 0] == float("inf")).all() and (row[sign < 0] == -float("inf")).all()
+        rest = [m for m in range(M) if m != M // 2]
+        assert torch.equal(y[rest], clean[rest])

@@ -441,3 +441,39 @@ def test_packed_scales_and_zero_points(dev):
             setattr(ly, which, w)
             with pytest.raises(ops.NotCovered):
                 ly(x, 3)
+
+
+@pytest.mark.parametrize("kind,group", [("int8", 0), ("uint8", 64)])
+@pytest.mark.parametrize("T", [1, 7, 24])
+def test_one_signed_tokens_and_narrow_weights(dev, kind, group, T):
+    """Tokens of one sign (their sum over k is far from zero) and weights of a few steps around
+    zero, the zero points anywhere."""
+    E, H, I = 4, 4096, 256
+    g = torch.Generator("cuda").manual_seed(T)
+
+    def small(rows, K):
+        q = torch.randint(-3, 4, (E, rows, K), generator=g, device="cuda", dtype=torch.int16)
+        c = (0.75, 0.5) if K == H else (0.5, 0.25)  # scales that keep h near one
+        if kind == "int8":
+            s = (torch.rand(E, rows, generator=g, device="cuda") * c[0] + c[1]) * K ** -0.5
+            return q.to(torch.int8), s.half(), None
+        z = torch.randint(3, 253, (E, K // group, rows), generator=g, device="cuda",
+                          dtype=torch.int16)
+        W = (q + z.repeat_interleave(group, 1).transpose(1, 2)).to(torch.uint8)
+        s = (torch.rand(E, K // group, rows, generator=g, device="cuda") * c[0] + c[1]) * K ** -0.5
+        return W, s.half(), z.to(torch.uint8)
+
+    ly = Layer(kind, E, H, I, group, seed=T)
+    ly.gu, ly.dn = small(2 * I, H), small(H, I)
+    x = rand(T, H, seed=T).abs()
+    ids = torch.randint(0, E, (T, 2), generator=g, device="cuda").int()
+    w = torch.rand(T, 2, generator=g, device="cuda") + 0.5
+    y = ly.experts(x, ids, w)
+    # acc(K) counts K / 16 truncations of the whole sum; here at most a step of 64 k is added on the
+    # tensor core (20), the steps of a warp and the warps in fp32: K / 256 + 16 at 4 warps or more
+    full, L.acc = L.acc, lambda K: (20 + K / 256 + 16) * 2.0 ** -23
+    try:
+        ref, tol = ly.ref(x, ids, w)
+    finally:
+        L.acc = full
+    assert_close(y, ref, tol)
