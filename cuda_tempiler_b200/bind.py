@@ -22,6 +22,7 @@ import os
 import threading
 
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 
 from . import ops
@@ -126,12 +127,19 @@ def _stock_epilogue(y, activation, residual):
     return y if residual is None else y + residual
 
 
-def _fused(x, weight, bias, activation, residual, run):
-    """run(residual rows) where the epilogue kernels cover the extra operands, else None.  They
-    have no backward pass: with gradients to record the stock operators run."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias, residual)):
-        return None
+def _differentiated(*tensors) -> bool:
+    """Whether any of them takes part in reverse- or forward-mode differentiation, or in a
+    function transform (torch.func): the epilogue kernels have no rules for those."""
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and (grad and t.requires_grad or fwAD.unpack_dual(t).tangent is not None
+                              or torch._C._functorch.is_functorch_wrapped_tensor(t)):
+            return True
+    return False
+
+
+def _fused(x, weight, bias, residual, run):
+    """run(residual rows) where the epilogue kernels cover the extra operands, else None."""
     N = weight.shape[0]
     if residual is not None and residual.shape != (*x.shape[:-1], N):
         return None
@@ -153,14 +161,15 @@ def linear_fp16(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
                 residual: torch.Tensor | None = None) -> torch.Tensor:
     """y = act(x @ weight^T (+ bias)) (+ residual) for x [..., K], weight [N, K], residual
     [..., N].  With an activation or a residual the kernels fuse the whole epilogue
-    (``ops.gemm_fp16_epilogue``); a bias alone is added to the rounded product."""
+    (``ops.gemm_fp16_epilogue``), unless a derivative is asked for; a bias alone is added to the
+    rounded product."""
     fuse = activation not in (None, "none") or residual is not None
-    if enabled():
+    if enabled() and not (fuse and _differentiated(x, weight, bias, residual)):
         x2 = x.reshape(-1, x.shape[-1])
         if covered_fp16(x2, weight):
             N = weight.shape[0]
             if fuse:
-                y = _fused(x, weight, bias, activation, residual,
+                y = _fused(x, weight, bias, residual,
                            lambda res: ops.gemm_fp16_epilogue(x2, weight, bias, activation, res))
                 if y is not None:
                     _count("tempo")
@@ -194,13 +203,14 @@ def linear_w8a16(x: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
                  residual: torch.Tensor | None = None) -> torch.Tensor:
     """``linear_fp16`` with an 8-bit weight."""
     fuse = activation not in (None, "none") or residual is not None
-    if enabled():
+    if enabled() and not (fuse and _differentiated(x, W, scale, bias, residual)):
         x2 = x.reshape(-1, x.shape[-1])
         if covered_w8a16(x2, W, scale, zero, group_size):
             N = W.shape[0]
             if fuse:
-                y = _fused(x, W, bias, activation, residual, lambda res: ops.gemm_w8a16_epilogue(
-                    x2, W, scale, zero, group_size, bias, activation, res))
+                y = _fused(x, W, bias, residual,
+                           lambda res: ops.gemm_w8a16_epilogue(x2, W, scale, zero, group_size,
+                                                               bias, activation, res))
                 if y is not None:
                     _count("tempo")
                     return y.reshape(*x.shape[:-1], N)

@@ -426,3 +426,18 @@ def test_an_infinite_activation_times_8_bit_weights(dev, kind, group):
         assert (row[sign > 0] == float("inf")).all() and (row[sign < 0] == -float("inf")).all()
         rest = [m for m in range(M) if m != M // 2]
         assert torch.equal(y[rest], clean[rest])
+
+
+@pytest.mark.parametrize("kind,group", [("int8", 0), ("uint8", 64)])
+def test_linear_layers_keep_the_gradient_of_a_scale(dev, monkeypatch, kind, group):
+    from cuda_tempiler_b200 import bind
+    monkeypatch.setenv("TEMPO_KERNELS", "1")
+    W, s, z = weights(kind, 272, 512, group)
+    x, res = rand(8, 512, seed=4), rand(8, 272, seed=2)
+    grads = []
+    for on in ("1", "0"):
+        monkeypatch.setenv("TEMPO_KERNELS", on)
+        leaf = s.clone().requires_grad_()
+        bind.linear_w8a16(x, W, leaf, z, group, activation="silu", residual=res).sum().backward()
+        grads.append(leaf.grad)
+    assert torch.equal(*grads) and grads[0].abs().sum() > 0
