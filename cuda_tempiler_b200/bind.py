@@ -6,9 +6,10 @@ not cover a shape, and the whole thing behind an environment switch that is OFF 
 (``TEMPO_KERNELS=1`` turns it on).  This module is that template for PyTorch:
 
 * ``torch.ops.tempo.gemm_fp16(A, B)`` and ``torch.ops.tempo.gemm_w8a16(A, W, scale, zero,
-  group_size)`` are strict: they run the library's kernels or raise (``NotCovered`` for a shape
-  the dispatcher does not cover, RuntimeError for a CUDA error or a missing library).  They have
-  fake (meta) implementations, so they trace under torch.compile / export as opaque ops.
+  group_size)``, and with a bias, an activation and a residual ``gemm_fp16_epilogue`` and
+  ``gemm_w8a16_epilogue``, are strict: they run the library's kernels or raise (``NotCovered`` for
+  a shape the dispatcher does not cover, RuntimeError for a CUDA error or a missing library).  They
+  have fake (meta) implementations, so they trace under torch.compile / export as opaque ops.
 * ``linear_fp16`` / ``linear_w8a16`` are what a model's linear layer calls.  With the switch
   off they are the framework's stock path (``F.linear`` on the dequantised weight for W8A16);
   with it on they call the custom op when ``covered()`` says the shape is shipped and fall back
@@ -24,6 +25,7 @@ import threading
 import torch
 import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
+from torch._subclasses.fake_tensor import FakeTensor
 
 from . import ops
 from ._lib import NotCovered
@@ -76,9 +78,35 @@ def _(A, W, scale, zero, group_size):
     return A.new_empty((A.shape[0], W.shape[0]))
 
 
+@torch.library.custom_op("tempo::gemm_fp16_epilogue", mutates_args=())
+def gemm_fp16_epilogue(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | None,
+                       activation: str, residual: torch.Tensor | None) -> torch.Tensor:
+    """C = act(A @ B^T + bias) + residual, one rounding (``ops.gemm_fp16_epilogue``)."""
+    return ops.gemm_fp16_epilogue(A, B, bias, activation, residual)
+
+
+@gemm_fp16_epilogue.register_fake
+def _(A, B, bias, activation, residual):
+    return A.new_empty((A.shape[0], B.shape[0]))
+
+
+@torch.library.custom_op("tempo::gemm_w8a16_epilogue", mutates_args=())
+def gemm_w8a16_epilogue(A: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
+                        zero: torch.Tensor | None, group_size: int, bias: torch.Tensor | None,
+                        activation: str, residual: torch.Tensor | None) -> torch.Tensor:
+    """``tempo::gemm_fp16_epilogue`` with an 8-bit weight (kinds of ``tempo::gemm_w8a16``)."""
+    return ops.gemm_w8a16_epilogue(A, W, scale, zero, group_size, bias, activation, residual)
+
+
+@gemm_w8a16_epilogue.register_fake
+def _(A, W, scale, zero, group_size, bias, activation, residual):
+    return A.new_empty((A.shape[0], W.shape[0]))
+
+
 # ------------------------------------------------------------------------------ coverage
 def _aligned(t: torch.Tensor) -> bool:
-    return t.data_ptr() % 16 == 0
+    # under a trace there is no address yet: the strict op raises NotCovered if the real one is off
+    return isinstance(t, FakeTensor) or t.data_ptr() % 16 == 0
 
 
 def covered_fp16(x2: torch.Tensor, weight: torch.Tensor) -> bool:
@@ -130,12 +158,22 @@ def _stock_epilogue(y, activation, residual):
 def _differentiated(*tensors) -> bool:
     """Whether any of them takes part in reverse- or forward-mode differentiation, or in a
     function transform (torch.func): the epilogue kernels have no rules for those."""
-    grad = torch.is_grad_enabled()
-    for t in tensors:
-        if t is not None and (grad and t.requires_grad or fwAD.unpack_dual(t).tangent is not None
-                              or torch._C._functorch.is_functorch_wrapped_tensor(t)):
-            return True
-    return False
+    grad, dual = torch.is_grad_enabled(), fwAD._current_level >= 0
+    wrapped = torch._C._functorch.peek_interpreter_stack() is not None
+    if not (grad or dual or wrapped):
+        return False
+    return any(t is not None and (
+        grad and t.requires_grad or dual and fwAD.unpack_dual(t).tangent is not None
+        or wrapped and torch._C._functorch.is_functorch_wrapped_tensor(t)) for t in tensors)
+
+
+def _op(name: str, x):
+    """The strict function, or under a trace (fake tensors, a dispatch mode, torch.compile) its custom
+    op, which costs 17 us of host time a call (19 us without, 36 with)."""
+    if type(x) in (torch.Tensor, torch.nn.Parameter) and not torch._C._len_torch_dispatch_stack() \
+            and not torch.compiler.is_compiling():
+        return getattr(ops, name)
+    return getattr(torch.ops.tempo, name)
 
 
 def _fused(x, weight, bias, residual, run):
@@ -170,7 +208,8 @@ def linear_fp16(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
             N = weight.shape[0]
             if fuse:
                 y = _fused(x, weight, bias, residual,
-                           lambda res: ops.gemm_fp16_epilogue(x2, weight, bias, activation, res))
+                           lambda res: _op("gemm_fp16_epilogue", x2)(
+                               x2, weight, bias, activation or "none", res))
                 if y is not None:
                     _count("tempo")
                     return y.reshape(*x.shape[:-1], N)
@@ -209,8 +248,8 @@ def linear_w8a16(x: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
             N = W.shape[0]
             if fuse:
                 y = _fused(x, W, bias, residual,
-                           lambda res: ops.gemm_w8a16_epilogue(x2, W, scale, zero, group_size,
-                                                               bias, activation, res))
+                           lambda res: _op("gemm_w8a16_epilogue", x2)(
+                               x2, W, scale, zero, group_size, bias, activation or "none", res))
                 if y is not None:
                     _count("tempo")
                     return y.reshape(*x.shape[:-1], N)

@@ -7,7 +7,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 from cuda_tempiler_b200 import bind, ops
 
-pytestmark = pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+pytestmark = pytest.mark.filterwarnings("error:Accessing the data pointer of FakeTensor")
 M, N, K = 6, 48, 128
 
 
@@ -97,3 +97,25 @@ def test_function_transforms_take_the_stock_path(monkeypatch):
     assert torch.allclose(torch.func.vmap(lambda a, r: bind.linear_fp16(
         a[None], W, activation="silu", residual=r[None])[0])(x, res), y, rtol=2.0 ** -9,
                           atol=2.0 ** -9)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "int8", "uint8"])
+def test_fused_layers_trace_as_opaque_ops(fake, kind):
+    x, w, bias, res = operands(kind)
+    for b, r in ((bias, res), (None, None), (bias, None), (None, res)):
+        y, routes = layer(kind, x, w, b, r)
+        assert routes == {"tempo": 1, "fallback": 0}
+        assert y.shape == (M, N) and y.dtype == torch.float16 and y.is_cuda
+
+
+def test_fused_layers_in_a_traced_graph(monkeypatch):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    monkeypatch.setenv("TEMPO_KERNELS", "1")
+    with FakeTensorMode():
+        x, w, bias, res = operands("uint8")
+
+        def f(x, res):
+            return bind.linear_w8a16(x, *w, bias=bias, activation="gelu", residual=res)
+        graph = make_fx(f)(x, res).graph
+    assert [n.target for n in graph.nodes if n.op == "call_function"
+            and "tempo" in str(n.target)] == [torch.ops.tempo.gemm_w8a16_epilogue.default]

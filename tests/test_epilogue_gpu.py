@@ -441,3 +441,29 @@ def test_linear_layers_keep_the_gradient_of_a_scale(dev, monkeypatch, kind, grou
         bind.linear_w8a16(x, W, leaf, z, group, activation="silu", residual=res).sum().backward()
         grads.append(leaf.grad)
     assert torch.equal(*grads) and grads[0].abs().sum() > 0
+
+
+def test_fused_layers_under_a_trace(dev, monkeypatch):
+    """The custom ops a trace records give what the layers give, and keep their fake shapes."""
+    from cuda_tempiler_b200 import bind
+    from torch.fx.experimental.proxy_tensor import make_fx
+    monkeypatch.setenv("TEMPO_KERNELS", "1")
+    x, res, bias = rand(6, 512, seed=1), rand(6, 272, seed=2), rand(272, seed=3)
+    for kind, group in (("fp16", 0), ("int8", 0), ("uint8", 64)):
+        w = weights(kind, 272, 512, group)
+
+        def f(x, res):
+            if kind == "fp16":
+                return bind.linear_fp16(x, w[0], bias, activation="silu", residual=res)
+            return bind.linear_w8a16(x, *w, group, bias, activation="silu", residual=res)
+        y = f(x, res)
+        for mode in ("real", "fake"):
+            bind.route_counts(reset=True)
+            traced = make_fx(f, tracing_mode=mode, _allow_non_fake_inputs=True)(x, res)
+            assert bind.route_counts()["tempo"] >= 1
+            assert any("epilogue" in str(n.target) for n in traced.graph.nodes)
+            assert torch.equal(traced(x, res), y)
+    args = (x, weights("fp16", 272, 512, 0)[0], bias, "relu", res)
+    torch.library.opcheck(torch.ops.tempo.gemm_fp16_epilogue, args)
+    W, s, z = weights("uint8", 272, 512, 64)
+    torch.library.opcheck(torch.ops.tempo.gemm_w8a16_epilogue, (x, W, s, z, 64, None, "none", res))
