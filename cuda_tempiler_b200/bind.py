@@ -186,12 +186,24 @@ def _fused(x, weight, bias, residual, run):
                             or res.stride(1) != 1 or res.stride(0) % 8 or not _aligned(res)):
         return None
     if bias is not None and (bias.dtype != torch.float16 or bias.device != x.device
-                             or not bias.is_contiguous() or not _aligned(bias)):
+                             or bias.shape != (N,) or not bias.is_contiguous()
+                             or not _aligned(bias)):
         return None
     try:
         return run(res)
     except NotCovered:
         return None
+
+
+def _scales_fit(x, W, scale, zero, group_size) -> bool:
+    """Whether scale and zero point have the types and shapes the kernels read."""
+    N, K = W.shape
+    group = W.dtype == torch.uint8
+    want = (K // group_size, N) if group else (N,)
+    if scale.dtype != torch.float16 or scale.shape != want or scale.device != x.device:
+        return False
+    return not group or (zero.dtype == torch.uint8 and zero.shape == want
+                         and zero.device == x.device)
 
 
 def linear_fp16(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -247,9 +259,11 @@ def linear_w8a16(x: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
         if covered_w8a16(x2, W, scale, zero, group_size):
             N = W.shape[0]
             if fuse:
-                y = _fused(x, W, bias, residual,
-                           lambda res: _op("gemm_w8a16_epilogue", x2)(
-                               x2, W, scale, zero, group_size, bias, activation or "none", res))
+                y = None
+                if _scales_fit(x, W, scale, zero, group_size):
+                    y = _fused(x, W, bias, residual,
+                               lambda res: _op("gemm_w8a16_epilogue", x2)(
+                                   x2, W, scale, zero, group_size, bias, activation or "none", res))
                 if y is not None:
                     _count("tempo")
                     return y.reshape(*x.shape[:-1], N)

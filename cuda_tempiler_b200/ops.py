@@ -383,6 +383,7 @@ def gemm_w8a16_epilogue(A: torch.Tensor, W: torch.Tensor, scale: torch.Tensor,
     N, k = W.shape
     if k != K:
         raise ValueError(f"K mismatch: A {tuple(A.shape)} W {tuple(W.shape)}")
+    scale, zero = (None if t is None else t.contiguous() for t in (scale, zero))
     _check_scales("W", (), N, K, kind, group_size, scale, zero)
     act, ldr = _epilogue_args(N, M, bias, activation, residual)
     dev = A.device

@@ -119,3 +119,22 @@ def test_fused_layers_in_a_traced_graph(monkeypatch):
         graph = make_fx(f)(x, res).graph
     assert [n.target for n in graph.nodes if n.op == "call_function"
             and "tempo" in str(n.target)] == [torch.ops.tempo.gemm_w8a16_epilogue.default]
+
+
+def test_operands_that_only_the_stock_path_takes(fake, monkeypatch):
+    """A bias or a residual that broadcasts, scales of another type or layout: the layer computes
+    them in either setting of the switch."""
+    refuse(monkeypatch)
+    monkeypatch.setattr(bind, "_op", lambda name, x: getattr(ops, name))
+    x, w, bias, res = operands("fp16")
+    for b, r in ((half(1), res), (half(1, N), res), (half(M, N), res), (bias, half(N)),
+                 (bias, half(M, 1)), (bias, half(1, N))):
+        y, routes = layer("fp16", x, w, b, r)
+        assert routes["fallback"] == 1 and y.shape == (M, N)
+    for kind in ("int8", "uint8"):
+        x, w, bias, res = operands(kind)
+        for i in (1, 2) if kind == "uint8" else (1,):
+            v = list(w)
+            v[i] = w[i].float()
+            y, routes = layer(kind, x, v, bias, res)
+            assert routes["fallback"] == 1 and y.shape == (M, N)

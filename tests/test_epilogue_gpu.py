@@ -467,3 +467,28 @@ def test_fused_layers_under_a_trace(dev, monkeypatch):
     torch.library.opcheck(torch.ops.tempo.gemm_fp16_epilogue, args)
     W, s, z = weights("uint8", 272, 512, 64)
     torch.library.opcheck(torch.ops.tempo.gemm_w8a16_epilogue, (x, W, s, z, 64, None, "none", res))
+
+
+@pytest.mark.parametrize("M", [3, 40])
+def test_scales_laid_out_as_for_the_plain_gemm(dev, monkeypatch, M):
+    """Scales and zero points with other values between theirs, taken as gemm_w8a16 takes them."""
+    from cuda_tempiler_b200 import bind, ops
+    monkeypatch.setenv("TEMPO_KERNELS", "1")
+    A = rand(M, 512, seed=1)
+    for kind, group in (("int8", 0), ("uint8", 64)):
+        W, s, z = weights(kind, 272, 512, group)
+        want = ops.gemm_w8a16_epilogue(A, W, s, z, group, activation="relu")
+        wide = torch.stack([s, s], -1).flatten(-2)[..., ::2]
+        zt = None if z is None else z.t().contiguous().t()
+        assert not wide.is_contiguous()
+        assert torch.equal(ops.gemm_w8a16_epilogue(A, W, wide, zt, group, activation="relu"), want)
+        bind.route_counts(reset=True)
+        assert torch.equal(bind.linear_w8a16(A, W, wide, zt, group, activation="relu"), want)
+        assert bind.route_counts()["tempo"] == 1
+        # types that only the stock path takes, and a bias that broadcasts
+        bias = rand(1, seed=3)
+        y = bind.linear_w8a16(A, W, s.float(), z, group, bias, activation="relu")
+        assert bind.route_counts()["fallback"] == 1
+        monkeypatch.setenv("TEMPO_KERNELS", "0")
+        assert torch.equal(y, bind.linear_w8a16(A, W, s.float(), z, group, bias, activation="relu"))
+        monkeypatch.setenv("TEMPO_KERNELS", "1")
