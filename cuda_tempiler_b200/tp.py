@@ -206,6 +206,36 @@ def _rank(group) -> int:
     return dist.get_rank(group) if dist.is_available() and dist.is_initialized() else 0
 
 
+def _adds_residual(group, all_reduce) -> bool | None:
+    """Whether this rank's partial takes the residual: rank 0's of those that are summed over, the
+    reducer's own group where it has one (``PeerAllReduce``).  None: a callable whose ranks are not
+    known, so the residual has to be added behind the sum."""
+    if callable(all_reduce):
+        if hasattr(all_reduce, "group"):
+            group = all_reduce.group
+        elif group is None:
+            return None
+    return _rank(group) == 0
+
+
+def _check_residual(residual, x, H: int, kernels: bool) -> None:
+    """On every rank, before anything runs: one that raised alone would leave the others in the
+    all-reduce."""
+    if residual.shape != (*x.shape[:-1], H):
+        raise ValueError(f"residual: expected {(*x.shape[:-1], H)}, got {tuple(residual.shape)}")
+    if kernels and (residual.dtype != torch.float16 or residual.device != x.device):
+        raise ValueError(f"residual: expected float16 on {x.device}, got {residual.dtype} on "
+                         f"{residual.device}")
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy in the layout the epilogue reads: rows of 16-byte vectors."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] \
+            and t.data_ptr() % 16 == 0:
+        return t
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
 def _down_residual(h, w, s, residual):
     """The down GEMM with the residual in its epilogue."""
     from . import ops
@@ -229,8 +259,13 @@ def mlp_forward(x: torch.Tensor, shard: MLPShard, group=None, gemm=None, swiglu=
     """y = down(silu(gate(x)) * up(x)) for this rank's shard, summed over the group.  With the
     library's own GEMM (gemm None) and an interleaved shard the fused gate_up + SwiGLU kernel
     runs where it covers M; ``fused=False`` keeps the two-kernel path.  ``residual`` [M, H] is added
-    once: by rank 0 to its partial, in the down GEMM's epilogue."""
+    once: by rank 0 of the ranks summed over to its partial, in the down GEMM's epilogue; behind the
+    sum where ``all_reduce`` is a callable without a ``group`` and none is given here."""
     own_gemm = gemm is None
+    adds = False
+    if residual is not None:
+        _check_residual(residual, x, shard.w_down.shape[0], own_gemm)
+        adds = _adds_residual(group, all_reduce)
     if fused is None:
         fused = _default_fused if gemm is None else False
     gemm = gemm or _default_gemm
@@ -239,14 +274,14 @@ def mlp_forward(x: torch.Tensor, shard: MLPShard, group=None, gemm=None, swiglu=
     if h is None:
         gu = gemm(x, shard.w_gate_up, shard.s_gate_up)   # [M, 2 I/tp]
         h = swiglu(gu, shard.gu_block)                    # [M, I/tp]
-    if residual is not None and _rank(group) == 0:
-        if own_gemm:
-            y = _down_residual(h, shard.w_down, shard.s_down, residual)
-        else:
-            y = gemm(h, shard.w_down, shard.s_down) + residual
+    if adds and own_gemm:
+        y = _down_residual(h, shard.w_down, shard.s_down, _rows16(residual))
     else:
         y = gemm(h, shard.w_down, shard.s_down)           # [M, H] partial
-    return _sum_partial(y, group, all_reduce)
+        if adds:
+            y = y + residual
+    y = _sum_partial(y, group, all_reduce)
+    return y + residual if adds is None else y
 
 
 @dataclass
@@ -281,10 +316,17 @@ def moe_forward(x: torch.Tensor, w_router: torch.Tensor, shard: MoEShard, top_k:
                 residual: torch.Tensor | None = None) -> torch.Tensor:
     """The mixture-of-experts layer of ``ops.moe_layer`` over the ranks of the group: every rank
     routes (the router is not sharded), runs its slice of the chosen experts, and the fp16 partials
-    are summed; ``residual`` is added by rank 0."""
+    are summed; ``residual`` is added once, as ``mlp_forward`` adds it."""
+    adds = False
+    if residual is not None:
+        _check_residual(residual, x, shard.w_down.shape[1], layer is None)
+        adds = _adds_residual(group, all_reduce)
+        if adds and layer is None:
+            residual = _rows16(residual)
     layer = layer or _default_layer
-    y = layer(x, w_router, shard, top_k, normalize, residual if _rank(group) == 0 else None)
-    return _sum_partial(y, group, all_reduce)
+    y = layer(x, w_router, shard, top_k, normalize, residual if adds else None)
+    y = _sum_partial(y, group, all_reduce)
+    return y + residual if adds is None else y
 
 
 class MLPGraph:

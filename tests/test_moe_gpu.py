@@ -477,3 +477,28 @@ def test_one_signed_tokens_and_narrow_weights(dev, kind, group, T):
     finally:
         L.acc = full
     assert_close(y, ref, tol)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "int8"])
+def test_tensor_parallel_residuals_in_any_layout(dev, kind):
+    """One that the epilogue does not read as it lies is laid out first: a rank must not raise
+    where the others go on to the all-reduce."""
+    from cuda_tempiler_b200 import tp
+    H, I, E, M = 256, 128, 4, 5
+    gu, dn = expert_weights(kind, E, 2 * I, H, 0, 7), expert_weights(kind, E, H, I, 0, 8)
+    x = whole(M, H, seed=9)
+    one = lambda t: None if t is None else t[0]  # noqa: E731
+    m = tp.MLPShard(gu[0][0], one(gu[1]), dn[0][0], one(dn[1]), I)
+    e = tp.MoEShard(gu[0], gu[1], dn[0], dn[1])
+    wr = router_weights(E, H, 11)
+    buf = rand(M + 1, H + 16, seed=12)
+    for res in (buf[:M, 3:3 + H], buf[1:2, 8:8 + H].expand(M, H), rand(H, M, seed=13).t()):
+        flat = res.contiguous()
+        assert torch.equal(tp.mlp_forward(x, m, residual=res), tp.mlp_forward(x, m, residual=flat))
+        assert torch.equal(tp.moe_forward(x, wr, e, 2, residual=res),
+                           tp.moe_forward(x, wr, e, 2, residual=flat))
+    for bad in (buf[:M, :H].float(), buf[:M, :H].cpu(), buf[:M, :H + 8], buf[0, :H]):
+        with pytest.raises(ValueError, match="residual"):
+            tp.mlp_forward(x, m, residual=bad)
+        with pytest.raises(ValueError, match="residual"):
+            tp.moe_forward(x, wr, e, 2, residual=bad)
