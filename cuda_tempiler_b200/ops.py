@@ -284,6 +284,17 @@ def _span(t: torch.Tensor) -> tuple:
     return a, a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
+def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Column ranges of one buffer: rows at the same distance whose bytes do not meet."""
+    if a.dim() != 2 or b.dim() != 2 or a.stride(1) != 1 or b.stride(1) != 1:
+        return False
+    (ea, eb), ld = (a.element_size(), b.element_size()), a.stride(0) * a.element_size()
+    if ld <= 0 or ld != b.stride(0) * eb:
+        return False
+    d = (b.data_ptr() - a.data_ptr()) % ld
+    return a.shape[1] * ea <= d and d + b.shape[1] * eb <= ld
+
+
 def _check_alias(out: torch.Tensor, residual: torch.Tensor | None, **inputs) -> None:
     """out may be the residual itself; any other overlap would be read after it is written."""
     lo, hi = _span(out)
@@ -291,7 +302,7 @@ def _check_alias(out: torch.Tensor, residual: torch.Tensor | None, **inputs) -> 
         if t is None:
             continue
         a, b = _span(t)
-        if a < hi and lo < b:
+        if a < hi and lo < b and not _interleaved(out, t):
             if name == "residual" and a == lo and t.stride() == out.stride():
                 continue
             raise ValueError(f"out overlaps {name}")

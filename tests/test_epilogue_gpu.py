@@ -492,3 +492,18 @@ def test_scales_laid_out_as_for_the_plain_gemm(dev, monkeypatch, M):
         monkeypatch.setenv("TEMPO_KERNELS", "0")
         assert torch.equal(y, bind.linear_w8a16(A, W, s.float(), z, group, bias, activation="relu"))
         monkeypatch.setenv("TEMPO_KERNELS", "1")
+
+
+@pytest.mark.parametrize("M", [4, 40, 500])
+def test_columns_of_one_buffer(dev, M):
+    """Activations, residual and output side by side in one buffer."""
+    from cuda_tempiler_b200 import ops
+    K, N = 256, 128
+    buf, W = rand(M, K + 2 * N, seed=1), rand(N, K, seed=2, scale=1 / 16)
+    A, res, out = buf[:, :K], buf[:, K:K + N], buf[:, K + N:]
+    keep = buf.clone()
+    want = ops.gemm_fp16_epilogue(A, W, residual=res)
+    assert ops.gemm_fp16_epilogue(A, W, residual=res, out=out) is out
+    assert torch.equal(out, want) and torch.equal(buf[:, :K + N], keep[:, :K + N])
+    with pytest.raises(ValueError, match="overlaps A"):
+        ops.gemm_fp16_epilogue(A, W, out=buf[:, K - 8:K - 8 + N])

@@ -162,6 +162,42 @@ def test_stock_path_of_the_linear_layers():
         bind.linear_fp16(x, w, activation="tanh", residual=r)
 
 
+def test_only_tensors_that_share_bytes_overlap():
+    """Against the sets of their bytes, for slices of one buffer."""
+    import itertools
+    from cuda_tempiler_b200 import ops
+    buf = torch.zeros(6, 32, dtype=torch.float16)
+    other = buf.view(torch.int8).view(6, 64)
+    flat = buf.view(-1)
+    slices = [buf[:, :16], buf[:, 16:], buf[:, 8:24], buf[:3, :16], buf[3:, :16], buf[2:5, 16:],
+              buf[1:4], buf[:, :8], buf[:, 24:], buf[2, 8:16], flat[10:20], other[:, 20:40],
+              other[:, :32], flat[:96].view(2, 48)[:, :16], buf[::2, :16], buf[1::2, :16]]
+
+    def bytes_of(t):
+        n, a = t.element_size(), t.data_ptr()
+        at = torch.zeros(t.shape, dtype=torch.int64)
+        for d, (size, st) in enumerate(zip(t.shape, t.stride())):
+            at += (torch.arange(size) * st).view([-1 if i == d else 1 for i in range(t.dim())])
+        return {a + int(x) * n + i for x in at.flatten() for i in range(n)}
+
+    refused_apart = []
+    for o, t in itertools.product(slices, slices):
+        if o.dim() != 2 or o.dtype != torch.float16:
+            continue
+        meet = bool(bytes_of(o) & bytes_of(t))
+        try:
+            ops._check_alias(o, None, A=t)
+            assert not meet, (o.shape, o.stride(), t.shape, t.stride())
+        except ValueError:
+            if not meet:
+                refused_apart.append((o.stride(), t.stride()))
+        same = o.data_ptr() == t.data_ptr() and o.stride() == t.stride()
+        if same:
+            ops._check_alias(o, t)  # the residual in place
+    # column slices of the same rows are told apart; other strides may be refused
+    assert all(a != b for a, b in refused_apart)
+
+
 def test_whole_warps_give_up_together():
     """Where all lanes of a warp wait and then act as a warp, the wait's outcome is the warp's
     (warp_wait) or the barrier group's (named_barrier_and); a lane that waits by itself does so
