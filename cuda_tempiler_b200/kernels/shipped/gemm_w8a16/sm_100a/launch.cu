@@ -100,10 +100,18 @@ bool make_map(CUtensorMap* m, const void* ptr, CUtensorMapDataType dt, int esize
   const cuuint64_t strides[1] = {ld * (uint64_t)esize};
   const cuuint32_t box[2] = {box_inner, box_outer};
   const cuuint32_t estr[2] = {1, 1};
-  if (fn(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-         CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return false;
+  auto encode = [&] {
+    return fn(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (!encode()) {
+    // A host thread that has made no runtime call yet has no current context, which the driver's
+    // encoder wants; setting its own device makes the device's primary context current.
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess || !encode())
+      return false;
+  }
   slot.key = key;
   slot.map = *m;
   slot.used = true;

@@ -507,3 +507,42 @@ def test_columns_of_one_buffer(dev, M):
     assert torch.equal(out, want) and torch.equal(buf[:, :K + N], keep[:, :K + N])
     with pytest.raises(ValueError, match="overlaps A"):
         ops.gemm_fp16_epilogue(A, W, out=buf[:, K - 8:K - 8 + N])
+
+
+@pytest.mark.parametrize("which", ["fp16 epilogue", "int8 epilogue", "plain fp16", "plain int8"])
+def test_first_call_of_a_host_thread(dev, which):
+    """A thread that has made no CUDA call yet: nothing is current in it."""
+    import threading
+
+    from cuda_tempiler_b200 import _lib
+    lib = _lib.load()
+    M, N, K = 40, 272, 64
+    kind = which.split()[0] if "epilogue" in which else which.split()[1]
+    A, w = rand(M, K, seed=1), weights(kind, N, K, 0)
+    out = poison(M, N)
+    st = torch.cuda.current_stream().cuda_stream
+    a, b, c = A.data_ptr(), w[0].data_ptr(), out.data_ptr()
+    s = None if w[1] is None else w[1].data_ptr()
+    torch.cuda.synchronize()
+    rc = []
+
+    def work():
+        if which == "fp16 epilogue":
+            rc.append(lib.tempo_sm100_gemm_fp16_epilogue(a, b, c, None, None, M, N, K, K, K, N, N, 0,
+                                                         None, 0, st))
+        elif which == "int8 epilogue":
+            rc.append(lib.tempo_sm100_gemm_w8a16_epilogue(a, b, s, None, c, None, None, M, N, K, K,
+                                                          K, N, N, 1, 0, 0, None, 0, st))
+        elif which == "plain fp16":
+            rc.append(lib.tempo_sm100_gemm_fp16(a, b, c, M, N, K, K, K, N, None, 0, st))
+        else:
+            rc.append(lib.tempo_sm100_gemm_w8a16(a, b, s, None, c, M, N, K, K, K, N, 1, 0, None, 0,
+                                                 st))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert rc == [0]
+    torch.cuda.synchronize()
+    check(out, A, w, 0, None, "none", None) if "epilogue" in which else None
+    assert torch.isfinite(out).all()
