@@ -222,6 +222,7 @@ int tempo_sm100_moe_layer(const void* x, const void* w_router, const void* bias,
   rc = moe_args(a, x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, residual, y, T, E,
                 H, I, top_k, ldx, ldr, ldy, weight_kind, group_size, gu_block, ws, ws_bytes);
   if (rc) return rc;
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e =
       launch_route({a.x, ldx, static_cast<const __half*>(w_router), ldw,
@@ -244,6 +245,7 @@ int tempo_sm100_moe_experts(const void* x, const int* ids, const float* weights,
       moe_args(a, x, w_gate_up, w_down, s_gate_up, z_gate_up, s_down, z_down, residual, y, T, E,
                H, I, top_k, ldx, ldr, ldy, weight_kind, group_size, gu_block, ws, ws_bytes);
   if (rc) return rc;
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = launch_ex(k_moe_plan, 1, kPlanThreads, 0, st, 1, ids,
                                   weights, T, top_k, E, a.plan);

@@ -5,7 +5,18 @@
 #include "../tempo/plugins/sm100/skeletons/gemm_sm100/kernel.cuh"
 #endif
 
+#include <cstdint>
+#include <mutex>
+
 namespace tempo_sm100 {
+
+// Held by an entry point while it enqueues: the launches of a call hand data on in the caller's
+// workspace, which host threads that share a stream may share too, so no other call's launch may get
+// between them.  One mutex per stream, up to collisions.
+inline std::mutex& launch_mutex(const void* stream) {
+  static std::mutex m[64];
+  return m[(reinterpret_cast<uintptr_t>(stream) >> 4) % 64];
+}
 
 constexpr int kStreamMaxM = 16;
 

@@ -76,6 +76,7 @@ int tempo_sm100_gemm_fp16_applicable(const void* A, const void* B, const void* C
 
 int tempo_sm100_gemm_fp16(const void* A, const void* B, void* C, int M, int N, int K, int lda,
                           int ldb, int ldc, void* ws, size_t ws_bytes, void* stream) {
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
   return tempo::gen::launch(fp16_params(A, B, C, M, N, K, lda, ldb, ldc, ws, ws_bytes),
                             static_cast<cudaStream_t>(stream));
 }
@@ -90,6 +91,7 @@ int tempo_sm100_gemm_w8a16_applicable(const void* A, const void* W, const void* 
 int tempo_sm100_gemm_w8a16(const void* A, const void* W, const void* scale, const void* zero,
                            void* C, int M, int N, int K, int lda, int ldw, int ldc, int quant_kind,
                            int group_size, void* ws, size_t ws_bytes, void* stream) {
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
   return tempo::gen::launch(w8_params(A, W, scale, zero, C, M, N, K, lda, ldw, ldc, quant_kind,
                                       group_size, ws, ws_bytes),
                             static_cast<cudaStream_t>(stream));
@@ -119,6 +121,7 @@ int tempo_sm100_gemm_hyperform(int weight_kind, const void* A, const void* W, co
     return cudaErrorInvalidConfiguration;
   }
   if (swap < 0 || swap > 2) return cudaErrorInvalidConfiguration;
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
   Hyper h{bn, swap, splits < 1 ? 1 : splits, group_m < 1 ? 1 : group_m, max_ctas};
   Problem pr{weight_kind, A, W, scale, zero, C, M, N, K, lda, ldw, ldc, group_size, ws, ws_bytes};
   return run(pr, h, static_cast<cudaStream_t>(stream));
@@ -140,6 +143,7 @@ int tempo_sm100_gemm_hyperform_cg(int weight_kind, const void* A, const void* W,
                             group_size)) {
     return cudaErrorInvalidConfiguration;
   }
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
   Hyper h{bn, 0, splits > 1 ? 2 : 1, group_m < 1 ? 1 : group_m, max_ctas};
   h.cta_group = 2;
   Problem pr{weight_kind, A, W, scale, zero, C, M, N, K, lda, ldw, ldc, group_size, ws, ws_bytes};
@@ -236,6 +240,7 @@ int tempo_sm100_gemm_w8a16_swiglu(const void* A, const void* W, const void* scal
       ldc < N / 2 || (ldc % 8))
     return cudaErrorInvalidConfiguration;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
   Problem pw{quant_kind, A, W, scale, zero, C, M, N, K, lda, ldw, ldc, group_size, ws, ws_bytes};
   // the copy after the counter prefix, which stays as the workspace's other users left it
   __half* wf = reinterpret_cast<__half*>(static_cast<char*>(ws) + kExpandOffset);
@@ -258,7 +263,9 @@ int tempo_sm100_gemm_fp16_epilogue(const void* A, const void* B, void* C, const 
   if (ws && !aligned16(ws)) return cudaErrorInvalidValue;
   Problem pr{0, A, B, nullptr, nullptr, C, M, N, K, lda, ldb, ldc, 0, ws, ws ? ws_bytes : 0};
   const int rc = fill_epilogue(pr, bias, residual, ldr, activation);
-  return rc ? rc : run_epilogue(pr, static_cast<cudaStream_t>(stream));
+  if (rc) return rc;
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
+  return run_epilogue(pr, static_cast<cudaStream_t>(stream));
 }
 
 int tempo_sm100_gemm_w8a16_epilogue(const void* A, const void* W, const void* scale,
@@ -273,7 +280,9 @@ int tempo_sm100_gemm_w8a16_epilogue(const void* A, const void* W, const void* sc
   Problem pr{quant_kind, A, W, scale, zero, C, M, N, K, lda, ldw, ldc, group_size, ws,
              ws ? ws_bytes : 0};
   const int rc = fill_epilogue(pr, bias, residual, ldr, activation);
-  return rc ? rc : run_epilogue(pr, static_cast<cudaStream_t>(stream));
+  if (rc) return rc;
+  const std::lock_guard<std::mutex> lock(launch_mutex(stream));
+  return run_epilogue(pr, static_cast<cudaStream_t>(stream));
 }
 
 int tempo_sm100_ipc_alloc(size_t bytes, void** out_ptr) {

@@ -146,8 +146,8 @@ int tempo_sm100_gemm_w8a16_swiglu(const void* A, const void* W, const void* scal
  * accumulator and one rounding to fp16.  Layouts, strides, coverage and return codes of
  * tempo_sm100_gemm_fp16 / tempo_sm100_gemm_w8a16; workspace as
  * tempo_sm100_epilogue_workspace_bytes says for the current device (zero-filled once like the
- * GEMMs', and interchangeable with theirs; less, or NULL, runs without, more slowly).  Calls that
- * can run at the same time need a workspace each.
+ * GEMMs', and interchangeable with theirs; less, or NULL, runs without, more slowly).  Calls on
+ * different streams need a workspace each; host threads may share a stream and its workspace.
  * Weights: fp16 and int8 enter exactly; a group-wise weight is rounded to fp16 above 16 rows, not
  * at all up to 16.  An infinite activation makes its own row infinite (NaN where the weight is 0).
  * bias: fp16 [N] or NULL.  residual: fp16 [M][N], row stride ldr elements, or NULL; it may be C

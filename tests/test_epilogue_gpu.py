@@ -546,3 +546,32 @@ def test_first_call_of_a_host_thread(dev, which):
     torch.cuda.synchronize()
     check(out, A, w, 0, None, "none", None) if "epilogue" in which else None
     assert torch.isfinite(out).all()
+
+
+def test_threads_on_one_stream(dev):
+    """Calls of several host threads on the same stream: the launches of one call and the workspace
+    they share stay together."""
+    import threading
+    shapes = [("fp16", 0, 90, 784, 4096), ("int8", 0, 200, 528, 4096), ("uint8", 128, 300, 528, 4096)]
+    jobs = []
+    for i, (kind, group, M, N, K) in enumerate(shapes):
+        A, w, res = rand(M, K, seed=i), weights(kind, N, K, group, seed=i), rand(M, N, seed=9 + i)
+        jobs.append((A, w, group, res, call(A, w, group, residual=res)))
+    bad = []
+
+    def work(i):
+        A, w, group, res, want = jobs[i]
+        try:
+            for _ in range(400):
+                if not torch.equal(call(A, w, group, residual=res), want):
+                    bad.append(i)
+        except Exception as e:
+            bad.append(e)
+
+    ts = [threading.Thread(target=work, args=(i % len(jobs),)) for i in range(6)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad, (len(bad), bad[:3])

@@ -502,3 +502,37 @@ def test_tensor_parallel_residuals_in_any_layout(dev, kind):
             tp.mlp_forward(x, m, residual=bad)
         with pytest.raises(ValueError, match="residual"):
             tp.moe_forward(x, wr, e, 2, residual=bad)
+
+
+def test_threads_on_one_stream(dev):
+    """A layer, its caller-routed form and GEMMs of several host threads on the same stream."""
+    import threading
+    from cuda_tempiler_b200 import ops
+    ly = Layer("int8", 16, 512, 256, seed=120)
+    x = rand(6, 512, seed=121)
+    y, ids, w = ly(x, 3, return_routing=True)
+    a, b, r = rand(300, 2048, seed=1), rand(784, 2048, seed=2, scale=0.02), rand(300, 784, seed=3)
+    c = torch.randint(-128, 128, (1024, 2048), device="cuda", dtype=torch.int8)
+    sc = torch.full((1024,), 1e-3, device="cuda", dtype=torch.float16)
+    calls = [lambda: ly(x, 3), lambda: ly.experts(x, ids, w),
+             lambda: ops.gemm_fp16_epilogue(a, b, residual=r), lambda: ops.gemm_fp16(a, b),
+             lambda: ops.gemm_w8a16(a.repeat(5, 1), c, sc)]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            for _ in range(300):
+                if not torch.equal(calls[i](), want[i]):
+                    bad.append(i)
+        except Exception as e:
+            bad.append(e)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad, bad
