@@ -575,3 +575,28 @@ def test_threads_on_one_stream(dev):
         t.join()
     torch.cuda.synchronize()
     assert not bad, (len(bad), bad[:3])
+
+
+@pytest.mark.parametrize("M", [4, 16, 64, 512])
+def test_tails_of_the_activations(dev, M):
+    """Small outputs of large negative arguments.  Relative to the value: the rounding to fp16, 2^-11;
+    of the exponential 2 + 1.2 |y| units of 2^-23 at the most, with y = -x (silu, -11 < x), -2 u
+    (gelu_tanh, u > -8) or -x^2 / 2 (gelu, -5.7 < x), each up to 16, before the result is below half
+    of fp16's smallest value: 22 units, 2^-18.5; as much for the tail's fit; argument and quotient
+    less than 8 units: 2^-17 covers them."""
+    from cuda_tempiler_b200 import ops
+    N, K = 512, 64
+    A = torch.zeros(M, K, dtype=torch.float16, device="cuda")
+    A[:, 0] = 1.0
+    B = torch.zeros(N, K, dtype=torch.float16, device="cuda")
+    B[:, 0] = torch.linspace(-9, 9, N, device="cuda").half()
+    x = B[:, 0].double()
+    for act in L.ACT:
+        y = ops.gemm_fp16_epilogue(A, B, activation=act).double()
+        if act == "gelu_tanh":  # without the cancellation of 1 + tanh
+            ref = x * torch.sigmoid(2 * (2 / torch.pi) ** 0.5 * (x + 0.044715 * x ** 3))
+        else:
+            ref = L.act(x, act)
+        tol = (L.U16 + 2.0 ** -17) * ref.abs() + 2.0 ** -25
+        bad = (y - ref).abs() > tol
+        assert not bad.any(), (act, int(bad.sum()), float(((y - ref).abs() / tol).max()))
