@@ -199,9 +199,9 @@ def test_only_tensors_that_share_bytes_overlap():
 
 
 def test_whole_warps_give_up_together():
-    """Where all lanes of a warp wait and then act as a warp, the wait's outcome is the warp's
-    (warp_wait) or the barrier group's (named_barrier_and); a lane that waits by itself does so
-    under `lane == 0`."""
+    """Where all lanes of a warp wait and then act as a warp, no lane leaves by its own wait's outcome:
+    the warp votes (warp_wait, __all_sync) or the barrier group does (named_barrier_and); a lane that
+    waits by itself does so under `lane == 0`."""
     import re
     from pathlib import Path
 
@@ -212,13 +212,17 @@ def test_whole_warps_give_up_together():
     roles = dict(zip(parts[1::2], parts[2::2]))
     assert list(roles) == ["TMA", "TMA: raw weights", "MMA", "epilogue", "unpacking"]
     for name, body in roles.items():
-        waits = re.findall(r"(\w*\(?\w*, ?\w*, ?)?\bmbar_wait\(", body)
+        waits = re.findall(r"\bmbar_wait\(", body)
         if name.startswith("TMA"):
             assert body.lstrip().startswith("if (lane == 0) {") and len(waits) == 1
         elif name == "epilogue":
             assert len(waits) == 1 and "named_barrier_and(bar, 128, mbar_wait(" in body
         else:
-            assert not waits and "warp_wait(" in body, name
+            own = re.findall(r"ok (?:&)?= mbar_wait\(", body)
+            assert len(own) == len(waits) and "ok = __all_sync(" in body.replace("if (!", "ok = ")
+            # every way out of the loops is a vote's
+            for line in body.splitlines():
+                assert "break;" not in line or re.search(r"if \(!(warp_wait|__all_sync)\(", line)
 
 
 # ------------------------------------------------------------------------------ sharding
