@@ -159,7 +159,8 @@ def _differentiated(*tensors) -> bool:
     """Whether any of them takes part in reverse- or forward-mode differentiation, or in a
     function transform (torch.func): the epilogue kernels have no rules for those."""
     grad, dual = torch.is_grad_enabled(), fwAD._current_level >= 0
-    wrapped = torch._C._functorch.peek_interpreter_stack() is not None
+    wrapped = not torch.compiler.is_compiling() \
+        and torch._C._functorch.peek_interpreter_stack() is not None
     if not (grad or dual or wrapped):
         return False
     return any(t is not None and (

@@ -138,3 +138,15 @@ def test_operands_that_only_the_stock_path_takes(fake, monkeypatch):
             v[i] = w[i].float()
             y, routes = layer(kind, x, v, bias, res)
             assert routes["fallback"] == 1 and y.shape == (M, N)
+
+
+def test_fused_layers_under_torch_compile(monkeypatch, recwarn):
+    """The counter's lock breaks the graph, as it does in a layer without an epilogue; nothing else
+    does, and the value is the layer's."""
+    monkeypatch.setenv("TEMPO_KERNELS", "1")
+    x, W, res = (torch.randn(*s).half() for s in ((M, K), (N, K), (M, N)))
+    torch._dynamo.reset()
+    y = torch.compile(lambda x: bind.linear_fp16(x, W, activation="silu", residual=res),
+                      backend="eager")(x)
+    assert torch.equal(y, bind.linear_fp16(x, W, activation="silu", residual=res))
+    assert not [w for w in recwarn if "does not know how to trace" in str(w.message)]
