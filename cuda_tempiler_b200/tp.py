@@ -298,7 +298,11 @@ class MoEShard:
 def shard_moe(w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, world: int,
               rank: int, s_gate=None, s_up=None, s_down=None) -> MoEShard:
     """Cut full expert weights (gate / up [E, I, H], down [E, H, I]) into rank `rank`'s slices: for
-    a few tokens every rank reads 1 / tp of each expert that is reached, whichever they are."""
+    a few tokens every rank reads 1 / tp of each expert that is reached, whichever they are.  fp16, or
+    int8 with a scale per output row; group-wise experts have no place here for their zero points."""
+    if torch.uint8 in (w_gate.dtype, w_up.dtype, w_down.dtype):
+        raise ValueError("group-wise (uint8) experts are not sharded: cut them by hand and call "
+                         "ops.moe_layer")
     sl = shard_rows(w_gate.shape[1], world, rank)
     sgu = None if s_gate is None else torch.cat([s_gate[:, sl], s_up[:, sl]], 1).contiguous()
     return MoEShard(torch.cat([w_gate[:, sl], w_up[:, sl]], 1).contiguous(), sgu,

@@ -114,3 +114,10 @@ def test_a_reducer_without_process_groups():
         y = tp.moe_forward(x, wr, s, 1, layer=_layer, all_reduce=lambda p: parts[0] + parts[1],
                            residual=res)
         assert torch.allclose(y, parts[0] + parts[1] + res, atol=1e-5)
+
+
+def test_group_wise_experts_are_refused():
+    from cuda_tempiler_b200 import tp
+    w, s = torch.zeros(2, 64, 64, dtype=torch.uint8), torch.ones(2, 1, 64).half()
+    with pytest.raises(ValueError, match="group-wise"):
+        tp.shard_moe(w, w, w, 1, 0, s, s, s)
