@@ -718,8 +718,8 @@ __device__ __forceinline__ int pow2_shift(unsigned amax_bits) {
 __device__ __forceinline__ float pow2f(int s) { return __int_as_float((127 + s) << 23); }
 
 // Rows of y are split like k_stream_linear's (CTA b: [H b / G, H (b + 1) / G)).  A warp walks the
-// steps of all slots as one sequence (warp w: steps w, w + 8, ...), so the weight stream does not
-// pause between experts; at a slot's end it adds its sums to its own fp32 sums per token in shared
+// steps of all slots as one sequence, of which it has one contiguous run, so the weight stream does
+// not pause between experts; at a slot's end it adds its sums to its own fp32 sums per token in shared
 // memory, which are added over the warps, in warp order, at the end.  The FIFO holds the fp32 h of
 // a slot's first 8 tokens; those of tokens 9-16, which few slots have, are read when used.
 template <int WQ, int MG, int RT>

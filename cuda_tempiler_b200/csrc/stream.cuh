@@ -422,15 +422,24 @@ struct LinearJob {
     for (int rt = 0; rt < RT; ++rt) r[rt] = p.n0 + rt * 16;
   }
   __device__ __forceinline__ void finish(const Piece& p, int rt, int mg, float4 v) const {
-    const float o[4] = {v.x, v.y, v.z, v.w};
+    const int n0 = p.n0 + rt * 16 + (lane >> 2), m0 = mg * 8 + 2 * (lane & 3);
+    float f[4] = {v.x, v.y, v.z, v.w};  // (n0, m0), (n0, m0 + 1), (n0 + 8, m0), (n0 + 8, m0 + 1)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = p.n0 + rt * 16 + (lane >> 2) + (j >= 2 ? 8 : 0);
-      const int m = mg * 8 + 2 * (lane & 3) + (j & 1);
-      if (n >= p.n1 || m >= a.M) continue;
+    for (int h = 0; h < 2; ++h) {
+      const int n = n0 + 8 * h;
+      if (n >= p.n1) continue;
       const float sc = WQ == kWInt8PerChannel ? __half2float(__ldg(a.scale + n)) : 1.f;
       const float b = a.epi.bias ? __half2float(__ldg(a.epi.bias + n)) : 0.f;
-      a.C[m * a.ldc + n] = __float2half_rn(epi_one(a.epi, o[j] * sc, b, m, n));
+      f[2 * h] = f[2 * h] * sc + b;
+      f[2 * h + 1] = f[2 * h + 1] * sc + b;
+    }
+    epi_act(f, a.epi.act);  // rows that do not exist too: once for all four
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + 4 * (j & 2), m = m0 + (j & 1);
+      if (n >= p.n1 || m >= a.M) continue;
+      if (a.epi.res) f[j] += __half2float(a.epi.res[m * a.epi.ldr + n]);
+      a.C[m * a.ldc + n] = __float2half_rn(f[j]);
     }
   }
 };

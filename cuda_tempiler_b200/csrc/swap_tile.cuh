@@ -545,7 +545,16 @@ struct SwapPlan {
 
 // How an M x N x K problem runs with mt tiles of activation rows, given ws_bytes of workspace, and
 // its cost in cycles.  Model of one k-block on one SM: its MMAs, its activations from L2 at
-// 64 B/cycle, its weights from HBM at 30 B/cycle of an SM and at 3400 of the GPU.
+// 64 B/cycle, its weights from HBM at 30 B/cycle of an SM and at 3400 of the GPU.  It ranks whole
+// tiles against equal shares and is no forecast of the time: the chain of barriers and issue, 400 to
+// 500 cycles a k-block, is left out on both sides.  Measured, whole / shares us (the
+// one chosen):
+//   fp16 100 x 15360 x 3840 24.3 / 29.7 (whole)   100 x 10240 x 5120 26.6 / 27.0 (shares)
+//        100 x 3840 x 15360 63.4 / 28.0 (shares)  333 x 18944 x 3840 49.4 / 56.7 (whole)
+//   int8 100 x 15360 x 3840 23.7 / 27.3 (whole)   100 x 10240 x 5120 29.5 / 25.0 (shares)
+//        100 x 3840 x 15360 68.6 / 25.8 (shares)  333 x 18944 x 3840 51.3 / 58.4 (whole)
+// Small problems with a long share of the fixed costs can go the wrong way: fp16 200 x 1024 x 1024
+// runs whole, 10.9 / 8.8.
 double epi_swap_cost(SwapPlan& p, int wkind, int M, int N, int K, int sms, size_t ws_bytes,
                      int mt) {
   const int want = (int)(((long long)M + mt - 1) / mt);

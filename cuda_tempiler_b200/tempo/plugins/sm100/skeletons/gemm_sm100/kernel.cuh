@@ -308,13 +308,6 @@ __device__ __forceinline__ void epi_row32(const EpiArgs& e, float (&f)[32], cons
   }
 }
 
-// One element (row m, column n) of the epilogue; b is bias[n] as a float (0 without a bias).
-__device__ __forceinline__ float epi_one(const EpiArgs& e, float v, float b, int m, int n) {
-  float f[1] = {v + b};
-  epi_act(f, e.act);
-  return e.res ? f[0] + __half2float(e.res[(long long)m * e.ldr + n]) : f[0];
-}
-
 template <int BN, int WQ, bool SWAP, bool SMEMDQ = false>
 __global__ void __launch_bounds__(SkelCfg<BN, WQ, SWAP, SMEMDQ>::THREADS, 1)
     k_gemm_sm100(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
