@@ -84,11 +84,10 @@ cudaError_t launch_big(void (*kern)(KArgs...), BigSmem& b, int max_smem, int gri
 }
 
 template <int WQ, int MG, int RT>
-cudaError_t launch_stream_rt(const LinearArgs& a, int grid, int ks, cudaStream_t st) {
+cudaError_t launch_stream_rt(const LinearArgs& a, int grid, cudaStream_t st) {
   using C = LinearCfg<WQ, MG, RT>;
   static BigSmem big;
-  return launch_big(k_stream_linear<WQ, MG, RT>, big, C::SMEM, grid, 32 * C::NW, C::SMEM, st, 1, a,
-                    ks);
+  return launch_big(k_stream_linear<WQ, MG, RT>, big, C::SMEM, grid, 32 * C::NW, C::SMEM, st, 1, a);
 }
 
 template <int WQ, int MG>
@@ -98,9 +97,9 @@ cudaError_t launch_stream_mg(const LinearArgs& a, cudaStream_t st) {
   // int8 M = 16, 35 rows: 15.4 us in 3 tiles, 22 in 2 pieces of 2, 20 as two workers.)
   const int grid = std::min(current_sms(), (a.N + 7) / 8);
   const int rows = (a.N + grid - 1) / grid;
-  if (rows <= 16) return launch_stream_rt<WQ, MG, 1>(a, grid, 16, st);
-  if (rows <= 32) return launch_stream_rt<WQ, MG, 2>(a, grid, 16, st);
-  return launch_stream_rt<WQ, MG, 3>(a, grid, 16, st);
+  if (rows <= 16) return launch_stream_rt<WQ, MG, 1>(a, grid, st);
+  if (rows <= 32) return launch_stream_rt<WQ, MG, 2>(a, grid, st);
+  return launch_stream_rt<WQ, MG, 3>(a, grid, st);
 }
 
 template <int WQ>

@@ -268,11 +268,11 @@ __device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red_
   const int n_mine = nsteps > warp ? ((nsteps - 1 - warp) >> (31 - __clz(KS))) + 1 : 0;
   bool more = n_mine > 0 && job.first(lp);
   const int rot = Job::ROTATE ? (int)((unsigned)nsteps * (unsigned)wk.id / (unsigned)wk.count) : 0;
-  int lstep = warp, lslot = 0;
-  auto issue = [&]() {
+  int lstep = warp;
+  auto issue = [&](int to) {  // the next step into slot `to`
     if (more) {
       const int step = lstep + rot;
-      job.copy(lp, step < nsteps ? step : step - nsteps, fifo + lslot * F::STAGE);
+      job.copy(lp, step < nsteps ? step : step - nsteps, fifo + to * F::STAGE);
       lstep += KS;
       if (lstep >= nsteps) {
         lstep = warp;
@@ -280,10 +280,9 @@ __device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red_
       }
     }
     cp_async_commit();  // one group per step, empty at the end: the wait below counts groups
-    lslot = lslot + 1 == S ? 0 : lslot + 1;
   };
 #pragma unroll 1
-  for (int i = 0; i < S - 1; ++i) issue();
+  for (int i = 0; i < S - 1; ++i) issue(i);
   int slot = 0;
   for (bool on = job.first(up); on; on = job.next(up)) {
     float acc[RT][MG][4] = {};
@@ -294,25 +293,30 @@ __device__ __forceinline__ void stream_run(Job& job, uint8_t* smem, float4* red_
     for (int j = 0; j < n_mine; ++j) {
       cp_async_wait<S - 2>();
       __syncwarp();  // every lane's copies of this step; every lane is done with the previous one
-      issue();
+      issue(slot ? slot - 1 : S - 1);
       const uint8_t* stage = fifo_p + slot * F::STAGE;
-      StreamA<WQ, RT> w;
-      stream_read_weights<WQ, RT>(w, stage, F::Z_OFF, z_row, lane);
+      uint32_t b[MG][1][St::NB];
 #pragma unroll
       for (int mg = 0; mg < MG; ++mg) {
         if (MG > 1 && !((live >> mg) & 1u)) continue;
-        uint32_t b[1][St::NB];
 #pragma unroll
         for (int v = 0; v < BV; ++v) {
           // a column that does not exist holds whatever the FIFO held: it stays in its column
           const uint4 x = lds16(stage + F::B_OFF + b_vec<BV>(mg, BV * (lane & 3) + v, lane >> 2));
-          b[0][4 * v] = x.x;
-          b[0][4 * v + 1] = x.y;
-          b[0][4 * v + 2] = x.z;
-          b[0][4 * v + 3] = x.w;
+          b[mg][0][4 * v] = x.x;
+          b[mg][0][4 * v + 1] = x.y;
+          b[mg][0][4 * v + 2] = x.z;
+          b[mg][0][4 * v + 3] = x.w;
         }
+      }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) stream_mma<WQ, RT, STEPS>(w, rt, b, acc[rt][mg]);
+      for (int rt = 0; rt < RT; ++rt) {  // one tile's operands in registers at a time
+        StreamA<WQ, 1> w;
+        const int zr[1] = {z_row[rt]};
+        stream_read_weights<WQ, 1>(w, stage + rt * 1024, F::Z_OFF + rt * 128 - rt * 1024, zr, lane);
+#pragma unroll
+        for (int mg = 0; mg < MG; ++mg)
+          if (MG == 1 || ((live >> mg) & 1u)) stream_mma<WQ, 1, STEPS>(w, 0, b[mg], acc[rt][mg]);
       }
       slot = slot + 1 == S ? 0 : slot + 1;
     }
@@ -460,12 +464,12 @@ struct LinearCfg {
 
 template <int WQ, int MG, int RT>
 __global__ void __launch_bounds__(32 * LinearCfg<WQ, MG, RT>::NW, 1)
-    k_stream_linear(const LinearArgs a, int ks) {
+    k_stream_linear(const LinearArgs a) {
   using C = LinearCfg<WQ, MG, RT>;
   extern __shared__ __align__(16) uint8_t smem[];
   pdl_wait();
   pdl_launch_dependents();
-  const StreamWorker wk = stream_worker<C::NW>(ks);
+  const StreamWorker wk = stream_worker<C::NW>(C::NW);
   LinearJob<WQ, MG, RT> job{a};
   split_even(a.N, wk.id, wk.count, job.lo, job.hi);
   job.npieces = (job.hi - job.lo + 16 * RT - 1) / (16 * RT);
