@@ -315,19 +315,20 @@ __global__ void __launch_bounds__(32 * RouteCfg<MG>::NW, 1) k_moe_route(const Ro
 // More than 32 tokens: a cluster of 8 CTAs routes 32 of them.  CTA r takes an eighth of k for all
 // experts, 128 at a time: warp (p, q) has 32 of the experts and every other 32-wide block of the
 // CTA's k range.  Its router weights go from L2 straight into the registers of the warp MMAs (no
-// other warp of the CTA wants them), 20 vectors in flight per thread; the tokens' part of k is in
+// other warp of the CTA wants them), 16 vectors in flight per thread; the tokens' part of k is in
 // shared memory.  The two sums of a logit are added, sent to the CTA that owns the token (t % 8)
 // and added there in rank order.  Every expert's sum has the same order, so equal router rows have
 // equal logits.  Two CTAs fit an SM for up to 200 experts.
 //
-// What bounds it is the chain of latencies of one cluster (12 us), not the 6.5 MB of 509 tokens,
-// E = 128, H = 5120: 16.5 us; with 16 warps that split k in four and one CTA per SM 21.5 (the
-// GPU then holds 13 or 14 clusters at a time); by clusters of 16 as above, 32 tokens each, 30.
+// What bounds it is the chain of latencies of one cluster, not the 6.5 MB of 509 tokens, E = 128,
+// H = 5120: 14.8 us (with 20 vectors in flight, some of them spilled, 16.3; E = 256, H = 7168 35 and
+// 41); with 16 warps that split k in four and one CTA per SM 21.5 (the GPU then holds 13 or 14
+// clusters at a time); by clusters of 16 as above, 32 tokens each, 30.
 constexpr int kManyTok = 32;
 constexpr int kManyCluster = 8;
 constexpr int kManySplit = 2;                        // warps that share a CTA's k
 constexpr int kManyThreads = 128 * kManySplit;
-constexpr int kManyRound = 5;                        // blocks of k a warp holds at once
+constexpr int kManyRound = 4;                        // blocks of k a warp holds at once (5: spills)
 constexpr int kManyBlocks = 20;                      // 32-wide blocks of k in shared memory
 constexpr int kManyRow = kManyBlocks * 64;           // bytes of a token's row there
 constexpr int kManyOwn = kManyTok / kManyCluster;
