@@ -36,19 +36,19 @@ namespace {
 // Up to kStreamMaxM rows: the stream while a CTA's share of the weight rows fits a piece or two
 // (every further piece reads the activations again and adds up its warps' sums), above that the
 // swapped tiles.  Measured, stream / swapped us at 8 and at 16 rows (N x K):
-//   fp16   3840 x 4096   8.5 / 11.1   9.2 / 11.3     5120 x 8192  18.1 / 18.5  21.5 / 18.7
-//          8192 x 3840  17.4 / 15.2  22.1 / 15.3    15360 x 3840  26.7 / 21.4  33.1 / 21.2
-//   int8   5120 x 8192  13.5 / 17.5  15.1 / 18.5     8192 x 3840  14.7 / 14.9  17.6 / 15.6
-//         10240 x 5120  18.6 / 19.6  21.1 / 20.2    15360 x 3840  22.3 / 20.0  25.9 / 20.3
-// Group-wise weights always (5120 x 8192 14.3 / 20.9 and 18.0 / 21.7, 15360 x 3840 23.6 / 25.9 and
-// 30.3 / 25.9): the stream takes them as they are, the tiles round each to fp16.
+//   fp16   3840 x 4096   7.4 / 11.2   8.3 / 11.1     5120 x 8192  17.5 / 19.2  21.0 / 19.6
+//          8192 x 3840  15.4 / 15.6  20.2 / 15.8    15360 x 3840  24.8 / 21.4  31.1 / 21.5
+//   int8   5120 x 8192  12.8 / 17.7  13.8 / 18.5     8192 x 3840  13.1 / 15.0  15.4 / 15.7
+//         10240 x 5120  17.2 / 19.6  19.0 / 20.3    15360 x 3840  20.4 / 20.3  23.3 / 20.5
+// Group-wise weights always (5120 x 8192 13.3 / 20.7 and 14.6 / 21.5, 15360 x 3840 20.5 / 25.7 and
+// 24.4 / 25.8): the stream takes them as they are, the tiles round each to fp16.
 bool stream_epilogue(int M, int N, int wkind) {
   if (M > kStreamMaxM) return false;
   const int sms = current_sms() > 0 ? current_sms() : 1;
   const int rows = (N + sms - 1) / sms;
   switch (wkind) {
     case kWFp16: return rows <= (M <= 8 ? 48 : 32);
-    case kWInt8PerChannel: return rows <= (M <= 8 ? 96 : 48);
+    case kWInt8PerChannel: return rows <= (M <= 8 ? 96 : 72);
     default: return true;
   }
 }

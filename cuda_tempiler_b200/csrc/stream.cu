@@ -93,8 +93,9 @@ cudaError_t launch_stream_rt(const LinearArgs& a, int grid, cudaStream_t st) {
 template <int WQ, int MG>
 cudaError_t launch_stream_mg(const LinearArgs& a, cudaStream_t st) {
   // One CTA per SM, 8 rows at least, as one worker in the fewest row tiles that hold its rows.
-  // (o_proj M = 1, 26 rows per CTA: 6.6 us in 2 tiles, 7.2 in 3, 8.7 as two workers of 8 warps;
-  // int8 M = 16, 35 rows: 15.4 us in 3 tiles, 22 in 2 pieces of 2, 20 as two workers.)
+  // (When this was chosen: o_proj M = 1, 26 rows per CTA, 6.6 us in 2 tiles, 7.2 in 3, 8.7 as two
+  // workers of 8 warps; int8 M = 16, 35 rows, 15.4 us in 3 tiles, 22 in 2 pieces of 2, 20 as two
+  // workers.  Now 6.4 and 13.8.)
   const int grid = std::min(current_sms(), (a.N + 7) / 8);
   const int rows = (a.N + grid - 1) / grid;
   if (rows <= 16) return launch_stream_rt<WQ, MG, 1>(a, grid, st);
