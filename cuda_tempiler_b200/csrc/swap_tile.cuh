@@ -12,11 +12,11 @@
 //
 // What bounds it: up to 128 rows the weights from HBM and 400 (fp16) to 500 (8-bit) cycles that a
 // k-block's chain of barriers and MMA issue takes; above, the activations' way from L2, 40 B per
-// cycle and SM.  Measured (us, floor in brackets): fp16 17 x 15360 x 3840 21.4 (18.2),
-// 100 x 15360 x 3840 24.0 (18.7), 256 x 18944 x 3840 36.5 (24.1), 333 x 18944 x 3840 45.5 (28.9);
-// int8 100 x 15360 x 3840 22.8 (9.6); uint8 333 x 5120 x 17408 62 (35.4), 51 of it here, the rest
-// k_swap_finish.  (A pair of CTAs per tile, cta_group::2 with half the activations each: the same
-// with fp16 weights, up to twice as long with 8-bit ones.)
+// cycle and SM.  Measured (us, floor in brackets): fp16 17 x 15360 x 3840 21.5 (18.2),
+// 100 x 15360 x 3840 23.8 (18.7), 256 x 18944 x 3840 37.6 (24.1), 333 x 18944 x 3840 47.6 (28.9);
+// int8 100 x 15360 x 3840 23.5 (9.6); uint8 333 x 5120 x 17408 65.4 (35.4), the time of
+// k_swap_finish behind it, about 10, included.  (A pair of CTAs per tile, cta_group::2 with half the
+// activations each: the same with fp16 weights, up to twice as long with 8-bit ones.)
 //
 // 8-bit weights: raw tiles in a ring of their own (released as soon as they are unpacked, so that
 // the HBM latency hides behind more bytes than the fp16 slots could hold); eight warps turn them
