@@ -42,19 +42,6 @@
 
 namespace tempo_sm100 {
 
-// Barrier `id` of `threads` threads; true when every one of them passed p.
-__device__ __forceinline__ bool named_barrier_and(int id, int threads, bool p) {
-  int r;
-  __syncwarp();
-  asm volatile(
-      "{\n\t.reg .pred q, o;\n\tsetp.ne.s32 q, %3, 0;\n\t"
-      "barrier.cta.red.and.pred o, %1, %2, q;\n\tselp.s32 %0, 1, 0, o;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(threads), "r"((int)p)
-      : "memory");
-  return r != 0;
-}
-
 // A bounded wait of a whole warp.  It may run out, or see the abort flag, in some lanes only: the
 // warp goes on or gives up as one, since what follows takes all of its lanes (elect.sync,
 // __syncwarp).  The loops over k-blocks vote less often, since until they do a wait that ran out

@@ -113,6 +113,19 @@ __device__ __forceinline__ void named_barrier_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// Barrier `id` of `threads` threads; true when every one of them passed p.
+__device__ __forceinline__ bool named_barrier_and(int id, int threads, bool p) {
+  int r;
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred q, o;\n\tsetp.ne.s32 q, %3, 0;\n\t"
+      "barrier.cta.red.and.pred o, %1, %2, q;\n\tselp.s32 %0, 1, 0, o;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"((int)p)
+      : "memory");
+  return r != 0;
+}
+
 // ---------------------------------------------------------------------------------------
 // TMA
 // ---------------------------------------------------------------------------------------
@@ -2149,7 +2162,9 @@ __global__ void __launch_bounds__(PairCfg<BN>::THREADS, 1)
       const int row0 = tp * 256 + (int)rank * 128 + quad * 32;
       EpiRes res;
       if (EPI && sg.contrib <= 1) res.load(args.epi, row0 + lane, args.rows_p, q0, args.rows_q);
-      if (!mbar_wait(tfull_bar(buf), uphase, abort_flag, 14)) break;
+      // one lane's wait may run out where another's did not: the TMEM loads below take whole warps,
+      // a tail's barriers all four, so all go on or none does
+      if (!named_barrier_and(1, 128, mbar_wait(tfull_bar(buf), uphase, abort_flag, 14))) break;
       tc_fence_after();
       const uint32_t t_acc = t_lane + buf * Cfg::ACC_STRIDE;
       if (sg.contrib > 1 && (args.ws == nullptr || args.counters == nullptr)) {

@@ -109,6 +109,19 @@ __device__ __forceinline__ void named_barrier_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// Barrier `id` of `threads` threads; true when every one of them passed p.
+__device__ __forceinline__ bool named_barrier_and(int id, int threads, bool p) {
+  int r;
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred q, o;\n\tsetp.ne.s32 q, %3, 0;\n\t"
+      "barrier.cta.red.and.pred o, %1, %2, q;\n\tselp.s32 %0, 1, 0, o;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"((int)p)
+      : "memory");
+  return r != 0;
+}
+
 // ---------------------------------------------------------------------------------------
 // TMA
 // ---------------------------------------------------------------------------------------

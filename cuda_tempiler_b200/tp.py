@@ -260,7 +260,8 @@ def mlp_forward(x: torch.Tensor, shard: MLPShard, group=None, gemm=None, swiglu=
     library's own GEMM (gemm None) and an interleaved shard the fused gate_up + SwiGLU kernel
     runs where it covers M; ``fused=False`` keeps the two-kernel path.  ``residual`` [M, H] is added
     once: by rank 0 of the ranks summed over to its partial, in the down GEMM's epilogue; behind the
-    sum where ``all_reduce`` is a callable without a ``group`` and none is given here."""
+    sum where ``all_reduce`` is a callable without a ``group`` and none is given here.  With
+    ``all_reduce=False`` the partials are the caller's to sum, rank 0 of ``group`` having added it."""
     own_gemm = gemm is None
     adds = False
     if residual is not None:

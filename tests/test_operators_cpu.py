@@ -225,6 +225,21 @@ def test_whole_warps_give_up_together():
                 assert "break;" not in line or re.search(r"if \(!(warp_wait|__all_sync)\(", line)
 
 
+def test_epilogue_warps_of_the_pair_tiles_give_up_together():
+    """The 2-CTA tiles that the epilogue GEMM runs on: all four warps or none."""
+    import re
+
+    from cuda_tempiler_b200 import build
+    text = (build.SKELETON / "kernel.cuh").read_text()
+    kernel = text[text.index("    k_gemm_sm100_pair(const"):text.index("// k_gemm_sm100_pair_w8: W8A16")]
+    epilogue = kernel[kernel.index("epilogue (both)"):]
+    waits = re.findall(r"[^\n]*\bmbar_wait\(", epilogue)
+    assert len(waits) == 1 and "named_barrier_and(1, 128, mbar_wait(" in waits[0]
+    others = kernel[:kernel.index("epilogue (both)")]
+    for role in re.split(r"// -{20,} ", others)[1:]:  # the producer's and the issuer's waits
+        assert "mbar_wait" not in role or "lane == 0) {" in role.split("mbar_wait")[0]
+
+
 # ------------------------------------------------------------------------------ sharding
 def _port():
     s = socket.socket()
